@@ -118,7 +118,8 @@ def _scale_of(largest, amax):
     top, exponent = math.frexp(largest)
     f, e = torch.frexp(amax)
     e = torch.where(amax > 0, e - exponent + (f > top), torch.full_like(e, -126)).clamp_min(-126)
-    return torch.ldexp(torch.ones_like(amax), e)
+    # its bits: a power function need not be exact
+    return ((e + 127) << 23).to(torch.int32).view(torch.float32)
 
 
 def _encode(x, fmt):
@@ -327,13 +328,18 @@ def work(case):
 # ---- the definition in 64 bits ------------------------------------------------
 
 
+def _power(e):
+    """2 ** e for whole numbers e, from its bits: a power function need not be exact."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
 def _value(byte, fmt):
     """What a byte stands for, from the format's definition."""
     byte = byte.long()
     if fmt == "int8":
         return torch.where(byte > 127, byte - 256, byte).double()
     exponent, mantissa = byte // 8 % 16, (byte % 8).double()
-    size = torch.where(exponent > 0, (8 + mantissa) * torch.pow(2.0, (exponent - 10).double()), mantissa * 2.0 ** -9)
+    size = torch.where(exponent > 0, (8 + mantissa) * _power(exponent - 10), mantissa * 2.0 ** -9)
     return torch.where(byte > 127, -size, size)
 
 
@@ -342,7 +348,7 @@ def _nearest(x, fmt):
     if fmt == "int8":
         return torch.round(x)
     _, e = torch.frexp(x)
-    step = torch.pow(2.0, (e.clamp_min(-5) - 4).double())
+    step = _power(e.clamp_min(-5) - 4)
     return torch.round(x / step) * step
 
 
@@ -384,7 +390,7 @@ def _exact_append(s):
                 here = x[max(0, at - pos):at + BLOCK - pos]
                 amax = here.abs().amax((0, 2)).clamp_min(1e-300)
                 # a logarithm is rounded: an exact power must not come out above itself
-                step = torch.pow(2.0, torch.ceil(torch.log2(amax / LARGEST[fmt]) - 1e-12).clamp_min(-126))
+                step = _power(torch.ceil(torch.log2(amax / LARGEST[fmt]) - 1e-12).clamp_min(-126))
                 if at < pos:
                     before = scale[at, :, which]
                     step = torch.maximum(step, before)
