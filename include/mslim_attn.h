@@ -440,6 +440,83 @@ int mslim_attn_logical_kv_sha256(void *ctx, int layers, int64_t tokens, int kv_h
                                  const int32_t *const *page_tables, int page_tokens,
                                  char *hex_out);
 
+/* ---- 8-bit paged K/V cache ---------------------------------------------------- */
+
+/* No reference counterpart: a cache of half the bytes of the BF16 pages, for
+ * callers that trade the exact K/V for twice the tokens per card and per
+ * second of decode.  Pages of page_tokens tokens (a power of two, 16..4096);
+ * 16 tokens of one kv head (a block) share one scale for K and one for V, and
+ * a byte stands for its format's value times the scale.
+ *   MSLIM_ATTN_FORMAT_E4M3: sign, 4 exponent and 3 mantissa bits, +-448.
+ *   MSLIM_ATTN_FORMAT_INT8: -127..127.
+ * head_dim is a multiple of 16, at most 256; q_heads any multiple of kv_heads.
+ * The pools are 16-byte aligned, the scales 8-byte, Q, K, V and output rows
+ * 16-byte.  The table is device memory, as are the positions; an entry that
+ * names no page of the pool (padding, -1) is allowed: nothing is written
+ * through it, rows read through it are zeros, and attention gives its tokens
+ * no weight. */
+#define MSLIM_ATTN_FORMAT_E4M3 4
+#define MSLIM_ATTN_FORMAT_INT8 5
+typedef struct {
+    void *k_pool;     /* bytes [pool_pages][kv_heads][page_tokens][head_dim] */
+    void *v_pool;     /* bytes [pool_pages][kv_heads][page_tokens / 16][4][head_dim][4]:
+                       * byte [g][d][i] of a block is dim d of its token 4 * g + i */
+    float *scales;    /* [pool_pages][kv_heads][page_tokens / 16][2]: K, V */
+    const int32_t *page_table; /* [batch][pages_per_seq] */
+    int64_t pool_pages;
+    int32_t pages_per_seq, page_tokens, kv_heads, head_dim;
+    int32_t format;   /* MSLIM_ATTN_FORMAT_E4M3 or _INT8 */
+    int32_t reserved; /* 0 */
+} mslim_attn_kv8_cache;
+
+/* RoPE of Q and K and the append of K and V to the 8-bit cache in one launch:
+ * row t of sequence b (q [batch][tokens][q_heads][head_dim], k and v [batch]
+ * [tokens][kv_heads][head_dim]) is at position positions[b] + t.  A decode
+ * step (tokens 1) and a prompt chunk (batch 1) are the same call.
+ *   Rotation: rotate-half, by the angle position * inverse frequency in 64
+ *   bits, cos and sin and the products in 32; q_out is rounded to BF16 once
+ *   and K not at all before its 8 bits.  (mslim_attn_rope_append takes the
+ *   angle in 32 bits and rounds cos, sin and both products to BF16.)  theta 0:
+ *   no rotation, K is stored as it comes, q and q_out are not used.
+ *   Scale of a block: the smallest power of two that covers the new rows and,
+ *   where rows before them lie in the same block, not below the block's scale;
+ *   the bytes of those rows are rounded again where it grows.  Rows behind the
+ *   new ones in the last block keep their bytes but no longer mean anything: a
+ *   sequence ends with its last appended row.
+ *   A value that is not finite makes its block's scale NaN: attention that
+ *   sees the block gives NaN until an append begins the block anew.
+ * A row at a position outside [0, pages_per_seq * page_tokens) is not stored.
+ * Sequences of one call must not share the pages they append to.  q_out must
+ * not alias an input.  batch at most MSLIM_ATTN_MAX_BATCH, batch * tokens at
+ * most 2^22. */
+int mslim_attn_rope_append_kv8(void *ctx, const mslim_attn_kv8_cache *cache, const void *q, const void *k,
+                               const void *v, void *q_out, int batch, int tokens, const int32_t *positions,
+                               int q_heads, float theta, int llama3_scaling, float factor,
+                               float low_freq_factor, float high_freq_factor, float original_max_position);
+
+/* Rows first[b] .. first[b] + tokens - 1 (device int32 [batch], NULL: from row
+ * 0) of every sequence back as BF16 rows [batch][tokens][kv_heads][head_dim]
+ * of K and of V: value times scale, rounded to BF16 (exact for scales that
+ * mslim_attn_rope_append_kv8 wrote).  Rows outside the table are zeros. */
+int mslim_attn_pages_gather_kv8(void *ctx, const mslim_attn_kv8_cache *cache, int batch, int tokens,
+                                const int32_t *first, void *k_rows, void *v_rows);
+
+/* mslim_attn_decode_paged over the 8-bit cache: q and out [batch][q_heads]
+ * [head_dim], seq_lens host [batch], each >= 0 and within the table.  A
+ * sequence of no tokens (a padded slot) gets zeros, and so does a row all of
+ * whose tokens have no page.  Scores and the softmax are in 32 bits; each
+ * probability is rounded to BF16 for its product with V, and the row sum adds
+ * the rounded ones. */
+int mslim_attn_decode_kv8(void *ctx, const mslim_attn_kv8_cache *cache, const void *q, void *out, int batch,
+                          const int32_t *seq_lens, int q_heads, float scale);
+
+/* mslim_attn_prefill_causal over the 8-bit cache, for a batch: the last
+ * `queries` tokens of each sequence, already appended, attend to it; row i of
+ * sequence b sees tokens 0 .. priors[b] + i (host int32 [batch], each >= 0).
+ * q and out [batch][queries][q_heads][head_dim]. */
+int mslim_attn_prefill_kv8(void *ctx, const mslim_attn_kv8_cache *cache, const void *q, void *out, int batch,
+                           int queries, const int32_t *priors, int q_heads, float scale);
+
 /* ---- ColdStore record frames ----------------------------------------------- */
 
 /* One ColdStore record to be made from a pool page: its header fields

@@ -1159,6 +1159,170 @@ int mslim_attn_pages_gather(void *ctx, const void *pool, const int32_t *page_tab
                      "page gather launch");
 }
 
+// ---- 8-bit paged K/V cache ----
+
+static_assert(mslim::kFormatE4m3 == MSLIM_ATTN_FORMAT_E4M3 && mslim::kFormatInt8 == MSLIM_ATTN_FORMAT_INT8,
+              "format codes of the C ABI and the launchers");
+
+static bool aligned(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// Checks a cache description and a call's batch and heads; fills *out.
+static int kv8_cache(const mslim_attn_kv8_cache *cache, int batch, mslim::Kv8Cache *out) {
+    if (!cache || !cache->k_pool || !cache->v_pool || !cache->scales || !cache->page_table)
+        return fail("8-bit cache needs non-null pools, scales and page table");
+    if (cache->format != MSLIM_ATTN_FORMAT_E4M3 && cache->format != MSLIM_ATTN_FORMAT_INT8)
+        return fail("8-bit cache format must be 4 (E4M3) or 5 (INT8)");
+    if (cache->head_dim < 16 || cache->head_dim % 16 || cache->head_dim > mslim::kKv8MaxDim)
+        return fail("8-bit cache head_dim must be a multiple of 16 up to 256");
+    if (!is_pow2(cache->page_tokens) || cache->page_tokens < 16 || cache->page_tokens > 4096)
+        return fail("page_tokens must be a power of two in 16..4096");
+    if (cache->kv_heads < 1 || cache->kv_heads > 16384 || cache->pages_per_seq < 1 || cache->pool_pages < 1 ||
+        cache->pool_pages > INT32_MAX)
+        return fail("8-bit cache needs 1..16384 kv_heads, pages_per_seq >= 1 and 1..2^31-1 pool_pages");
+    if (cache->reserved != 0) return fail("8-bit cache: reserved must be 0");
+    if ((int64_t)cache->pages_per_seq * cache->page_tokens > INT32_MAX - 64)
+        return fail("8-bit cache: the page table names more than 2^31 tokens");
+    if (!aligned(cache->k_pool, 16) || !aligned(cache->v_pool, 16) || !aligned(cache->scales, 8))
+        return fail("8-bit cache needs 16-byte aligned pools and 8-byte aligned scales");
+    if (batch < 1 || batch > MSLIM_ATTN_MAX_BATCH) return fail("8-bit cache batch must be 1..4096");
+    out->k = static_cast<uint8_t *>(cache->k_pool);
+    out->v = static_cast<uint8_t *>(cache->v_pool);
+    out->scales = cache->scales;
+    out->table = cache->page_table;
+    out->pool_pages = cache->pool_pages;
+    out->pages_per_seq = cache->pages_per_seq;
+    out->shift = 0;
+    while ((1 << out->shift) < cache->page_tokens) ++out->shift;
+    out->kv_heads = cache->kv_heads;
+    out->head_dim = cache->head_dim;
+    out->format = cache->format;
+    return 0;
+}
+
+static bool kv8_overlaps(const mslim_attn_kv8_cache *cache, const void *p) {
+    return p == cache->k_pool || p == cache->v_pool || p == cache->scales;
+}
+
+int mslim_attn_rope_append_kv8(void *ctx, const mslim_attn_kv8_cache *cache, const void *q, const void *k,
+                               const void *v, void *q_out, int batch, int tokens, const int32_t *positions,
+                               int q_heads, float theta, int llama3_scaling, float factor,
+                               float low_freq_factor, float high_freq_factor, float original_max_position) {
+    g_error.clear();
+    if (!ctx) return fail("null context");
+    mslim::Kv8AppendLaunch l{};
+    if (int rc = kv8_cache(cache, batch, &l.cache)) return rc;
+    if (tokens < 1 || (int64_t)batch * tokens > (1 << 22)) return fail("8-bit append needs 1..2^22 rows in all");
+    if (!k || !v || !positions) return fail("8-bit append needs non-null k, v and positions");
+    if (!aligned(k, 16) || !aligned(v, 16)) return fail("8-bit append needs 16-byte aligned rows");
+    if (!(theta >= 0.0f) || !std::isfinite(theta)) return fail("8-bit append: theta must be finite and >= 0");
+    l.rotate = theta > 0.0f;
+    if (l.rotate) {
+        if (!q || !q_out) return fail("8-bit append with a rotation needs non-null q and q_out");
+        if (q_heads < 1 || q_heads % cache->kv_heads || q_heads > 65536)
+            return fail("8-bit append: q_heads must be a multiple of kv_heads");
+        if (!aligned(q, 16) || !aligned(q_out, 16)) return fail("8-bit append needs 16-byte aligned rows");
+        if (q_out == q || q_out == k || q_out == v || kv8_overlaps(cache, q_out))
+            return fail("8-bit append: q_out must not alias an input or the cache");
+        if (llama3_scaling && (!(factor > 0.0f) || !(high_freq_factor > low_freq_factor) ||
+                               !(low_freq_factor > 0.0f) || !(original_max_position > 0.0f)))
+            return fail("invalid llama3 RoPE scaling parameters");
+        // Turns per position of every pair, in 64 bits: the inverse
+        // frequency theta^(-2f / head_dim), scaled by parts of the wavelength
+        // range where asked, over 2 pi.
+        const double two_pi = 6.28318530717958647692528676655900577;
+        for (int f = 0; f < cache->head_dim / 2; ++f) {
+            double inv = std::pow((double)theta, -2.0 * f / cache->head_dim);
+            if (llama3_scaling) {
+                const double wavelength = two_pi / inv;
+                if (wavelength > (double)original_max_position / low_freq_factor) {
+                    inv /= factor;
+                } else if (wavelength >= (double)original_max_position / high_freq_factor) {
+                    const double smooth = (original_max_position / wavelength - low_freq_factor) /
+                                          ((double)high_freq_factor - low_freq_factor);
+                    inv = (1.0 - smooth) * inv / factor + smooth * inv;
+                }
+            }
+            l.turns.turn[f] = inv / two_pi;
+        }
+    }
+    l.q = static_cast<const uint16_t *>(q);
+    l.k = static_cast<const uint16_t *>(k);
+    l.v = static_cast<const uint16_t *>(v);
+    l.q_out = static_cast<uint16_t *>(q_out);
+    l.positions = positions;
+    l.batch = batch; l.tokens = tokens; l.q_heads = q_heads;
+    if (mslim::kv8_append_workgroups(l) >= (1 << 24)) return fail("8-bit append: too many rows and heads for one call");
+    Context &c = *ctx_of(ctx);
+    Lock lock(c);
+    return check_hip(mslim::launch_kv8_append(l, c.stream), "8-bit append launch");
+}
+
+int mslim_attn_pages_gather_kv8(void *ctx, const mslim_attn_kv8_cache *cache, int batch, int tokens,
+                                const int32_t *first, void *k_rows, void *v_rows) {
+    g_error.clear();
+    if (!ctx) return fail("null context");
+    mslim::Kv8Cache kv;
+    if (int rc = kv8_cache(cache, batch, &kv)) return rc;
+    if (tokens < 1 || tokens > INT32_MAX - 64) return fail("8-bit gather needs at least one row");
+    if (!k_rows || !v_rows || !aligned(k_rows, 16) || !aligned(v_rows, 16))
+        return fail("8-bit gather needs non-null, 16-byte aligned rows");
+    if (k_rows == v_rows || kv8_overlaps(cache, k_rows) || kv8_overlaps(cache, v_rows))
+        return fail("8-bit gather: the rows must not alias each other or the cache");
+    Context &c = *ctx_of(ctx);
+    Lock lock(c);
+    return check_hip(mslim::launch_kv8_gather(kv, batch, tokens, first, static_cast<uint16_t *>(k_rows),
+                                              static_cast<uint16_t *>(v_rows), c.stream),
+                     "8-bit gather launch");
+}
+
+// Attention over the 8-bit cache of sequences with lens[b] tokens before
+// `more` appended ones, arguments that both entry points share checked here.
+static int kv8_attention(void *ctx, const mslim_attn_kv8_cache *cache, const void *q, void *out, int batch,
+                         int queries, const int32_t *lens, int more, int q_heads, float scale) {
+    if (!ctx) return fail("null context");
+    mslim::Kv8AttentionLaunch l{};
+    if (int rc = kv8_cache(cache, batch, &l.cache)) return rc;
+    if (!q || !out || !lens) return fail("8-bit attention needs non-null q, out and lengths");
+    if (!aligned(q, 16) || !aligned(out, 16)) return fail("8-bit attention needs 16-byte aligned rows");
+    if (q_heads < 1 || q_heads % cache->kv_heads || q_heads > 65536)
+        return fail("8-bit attention: q_heads must be a multiple of kv_heads");
+    if (out == q || kv8_overlaps(cache, out)) return fail("8-bit attention: out must not alias an input");
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail("8-bit attention scale must be finite and > 0");
+    if (queries < 1 || (int64_t)batch * queries * q_heads > (1 << 27))
+        return fail("8-bit attention needs 1..2^27 rows (queries of all heads) in all");
+    const int64_t room = (int64_t)cache->pages_per_seq * cache->page_tokens;
+    for (int b = 0; b < batch; ++b)
+        if (lens[b] < 0 || (int64_t)lens[b] + more > room)
+            return fail("8-bit attention: a length is negative or exceeds the page table row");
+    l.queries = queries; l.q_heads = q_heads; l.scale = scale;
+    Context &c = *ctx_of(ctx);
+    Lock lock(c);
+    // Launches of up to kKv8Batch sequences: their lengths travel in the
+    // kernel arguments, so every batch can be recorded into a graph.
+    const int64_t row = (int64_t)queries * q_heads * cache->head_dim;
+    for (int b0 = 0; b0 < batch; b0 += mslim::kKv8Batch) {
+        l.batch = std::min(mslim::kKv8Batch, batch - b0);
+        l.q = static_cast<const uint16_t *>(q) + b0 * row;
+        l.out = static_cast<uint16_t *>(out) + b0 * row;
+        l.cache.table = cache->page_table + (int64_t)b0 * cache->pages_per_seq;
+        for (int b = 0; b < l.batch; ++b) l.len[b] = lens[b0 + b] + more;
+        if (int rc = check_hip(mslim::launch_kv8_attention(l, c.stream), "8-bit attention launch")) return rc;
+    }
+    return 0;
+}
+
+int mslim_attn_decode_kv8(void *ctx, const mslim_attn_kv8_cache *cache, const void *q, void *out, int batch,
+                          const int32_t *seq_lens, int q_heads, float scale) {
+    g_error.clear();
+    return kv8_attention(ctx, cache, q, out, batch, 1, seq_lens, 0, q_heads, scale);
+}
+
+int mslim_attn_prefill_kv8(void *ctx, const mslim_attn_kv8_cache *cache, const void *q, void *out, int batch,
+                           int queries, const int32_t *priors, int q_heads, float scale) {
+    g_error.clear();
+    return kv8_attention(ctx, cache, q, out, batch, queries, priors, queries, q_heads, scale);
+}
+
 int mslim_attn_logical_kv_sha256(void *ctx, int layers, int64_t tokens, int kv_heads, int head_dim,
                                  const void *const *keys, const void *const *values,
                                  const int32_t *const *page_tables, int page_tokens,

@@ -334,6 +334,57 @@ hipError_t launch_pages_append(uint16_t *k_pool, uint16_t *v_pool, const int32_t
 hipError_t launch_pages_gather(const uint16_t *pool, const int32_t *page_table, int page_tokens,
                                int kv_heads, int head_dim, int64_t first_token, int64_t tokens,
                                uint16_t *rows_out, hipStream_t stream);
+// The 8-bit paged K/V cache (csrc/kv8.hip).  Blocks of kKv8Block tokens share
+// one scale per kv head for K and one for V; a byte stands for its format's
+// value times the scale.
+//   k       [pool_pages][kv_heads][page_tokens][head_dim]
+//   v       [pool_pages][kv_heads][page_tokens / 16][4][head_dim][4]: byte
+//           [g][d][i] of a block is dim d of its token 4 * g + i
+//   scales  [pool_pages][kv_heads][page_tokens / 16][2] (K, V)
+constexpr int kFormatE4m3 = 4, kFormatInt8 = 5;
+constexpr int kKv8Block = 16;
+constexpr int kKv8MaxDim = 256;
+struct Kv8Cache {
+    uint8_t *k, *v;
+    float *scales;
+    const int32_t *table;  // [batch][pages_per_seq]
+    int64_t pool_pages;
+    int pages_per_seq, shift;  // page_tokens = 1 << shift
+    int kv_heads, head_dim, format;
+};
+// Turns (periods) per position of the rotary pairs, in 64 bits.
+struct Kv8Turns {
+    double turn[kKv8MaxDim / 2];
+};
+struct Kv8AppendLaunch {
+    Kv8Cache cache;
+    const uint16_t *q, *k, *v;  // [batch][tokens][heads][head_dim]
+    uint16_t *q_out;            // rotating launches only
+    const int32_t *positions;   // [batch]
+    int batch, tokens, q_heads;
+    bool rotate;
+    Kv8Turns turns;
+};
+// Workgroups of the launch; fewer than 2^24.
+int64_t kv8_append_workgroups(const Kv8AppendLaunch &l);
+hipError_t launch_kv8_append(const Kv8AppendLaunch &l, hipStream_t stream);
+// Rows first[b] .. first[b] + tokens of every sequence as BF16
+// [batch][tokens][kv_heads][head_dim]; first null: from row 0.
+hipError_t launch_kv8_gather(const Kv8Cache &cache, int batch, int tokens, const int32_t *first, uint16_t *k_rows,
+                             uint16_t *v_rows, hipStream_t stream);
+// Attention of `queries` rows of each sequence over its cached tokens: row i
+// of a sequence of len tokens sees tokens <= len - queries + i.
+constexpr int kKv8Batch = 64;  // sequences of one launch: its tables travel in the arguments
+struct Kv8AttentionLaunch {
+    Kv8Cache cache;
+    const uint16_t *q;
+    uint16_t *out;  // [batch][queries][q_heads][head_dim], as q
+    int batch, queries, q_heads;
+    float scale;
+    int len[kKv8Batch];  // 0: nothing cached, the rows are zeros
+};
+hipError_t launch_kv8_attention(const Kv8AttentionLaunch &l, hipStream_t stream);
+
 // Canonical head-major serialisation of one layer tensor: tokens
 // [first, first+count) of kv head `head` into out[count][head_dim]
 // (dense token-major source when page_table is null).

@@ -27,6 +27,8 @@ OPT_PREFILL_SPLIT = 2
 OPT_PREFILL_POOL = 3
 DECODE_STATIC_SCRATCH_BYTES = 16 << 20      # mslim_attn_decode_paged_noalloc partials bound
 FORMAT_BF16, FORMAT_F16, FORMAT_F32 = 1, 2, 3  # gpu_backend.rs:258-262
+FORMAT_E4M3, FORMAT_INT8 = 4, 5  # the 8-bit paged K/V cache
+KV8_BLOCK = 16  # its tokens that share a scale
 ERR_NONFINITE = -2
 
 
@@ -82,6 +84,10 @@ EXPORTS = (
     "mslim_attn_pages_append",
     "mslim_attn_rope_append",
     "mslim_attn_pages_gather",
+    "mslim_attn_rope_append_kv8",
+    "mslim_attn_pages_gather_kv8",
+    "mslim_attn_decode_kv8",
+    "mslim_attn_prefill_kv8",
     "mslim_attn_logical_kv_sha256",
     "mslim_attn_record_frame_bytes",
     "mslim_attn_record_frames",
@@ -109,6 +115,25 @@ class PageRecord(C.Structure):
     """mslim_attn_page_record: header fields of one record and its pool page."""
     _fields_ = [("page_id", C.c_uint64), ("token_start", C.c_uint64), ("layer", C.c_uint32),
                 ("tokens", C.c_uint32), ("pool_page", C.c_int32), ("first_row", C.c_uint32)]
+
+
+class Kv8Cache(C.Structure):
+    """mslim_attn_kv8_cache: one layer's 8-bit paged K/V cache.  Takes device
+    tensors (kept alive here) or integer device pointers:
+      k_pool     bytes [pool_pages][kv_heads][page_tokens][head_dim]
+      v_pool     bytes [pool_pages][kv_heads][page_tokens / 16][4][head_dim][4]
+      scales     f32 [pool_pages][kv_heads][page_tokens / 16][2]
+      page_table int32 [batch][pages_per_seq]
+    """
+    _fields_ = [("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("scales", C.c_void_p), ("page_table", C.c_void_p),
+                ("pool_pages", C.c_int64), ("pages_per_seq", C.c_int32), ("page_tokens", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("format", C.c_int32), ("reserved", C.c_int32)]
+
+    def __init__(self, k_pool, v_pool, scales, page_table, pool_pages: int, pages_per_seq: int, page_tokens: int,
+                 kv_heads: int, head_dim: int, format: int):
+        super().__init__(_ptr(k_pool), _ptr(v_pool), _ptr(scales), _ptr(page_table), pool_pages, pages_per_seq,
+                         page_tokens, kv_heads, head_dim, format, 0)
+        self.tensors = (k_pool, v_pool, scales, page_table)
 
 
 class MslimAttnError(RuntimeError):
@@ -171,6 +196,10 @@ def library() -> C.CDLL:
         "mslim_attn_pages_append": (I, [P, P, P, P, I, I, I, I, I, P, P, P]),
         "mslim_attn_rope_append": (I, [P, P, P, P, P, P, P, P, I, I, I, P, I, I, I, F, I, F, F, F, F]),
         "mslim_attn_pages_gather": (I, [P, P, P, I, I, I, I64, I64, P]),
+        "mslim_attn_rope_append_kv8": (I, [P, P, P, P, P, P, I, I, P, I, F, I, F, F, F, F]),
+        "mslim_attn_pages_gather_kv8": (I, [P, P, I, I, P, P, P]),
+        "mslim_attn_decode_kv8": (I, [P, P, P, P, I, PI32, I, F]),
+        "mslim_attn_prefill_kv8": (I, [P, P, P, P, I, I, PI32, I, F]),
         "mslim_attn_logical_kv_sha256": (I, [P, I, I64, I, I, P, P, P, I, C.c_char_p]),
         "mslim_attn_record_frame_bytes": (I64, [I]),
         "mslim_attn_record_frames": (I, [P, P, P, I64, I, I, I, C.c_uint32, P, I, P]),
@@ -452,6 +481,34 @@ class Context:
         self._check("pages_gather", self._lib.mslim_attn_pages_gather(
             self._h, _ptr(pool), _ptr(page_table_row), page_tokens, kv_heads, head_dim,
             first_token, tokens, _ptr(rows_out)))
+
+    # ---- 8-bit paged K/V cache -------------------------------------------
+    def rope_append_kv8(self, cache: Kv8Cache, q, k, v, q_out, batch: int, tokens: int, positions, q_heads: int,
+                        theta: float, llama3_scaling: bool = False, factor: float = 1.0,
+                        low_freq_factor: float = 1.0, high_freq_factor: float = 2.0,
+                        original_max_position: float = 1.0) -> None:
+        """Rotate Q into q_out and K, and append K and V; theta 0 appends only."""
+        self._check("rope_append_kv8", self._lib.mslim_attn_rope_append_kv8(
+            self._h, C.byref(cache), _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), batch, tokens, _ptr(positions), q_heads,
+            theta, int(bool(llama3_scaling)), factor, low_freq_factor, high_freq_factor, original_max_position))
+
+    def pages_gather_kv8(self, cache: Kv8Cache, batch: int, tokens: int, first, k_rows, v_rows) -> None:
+        """BF16 K and V rows first[b] .. first[b] + tokens - 1 (first None: from row 0)."""
+        self._check("pages_gather_kv8", self._lib.mslim_attn_pages_gather_kv8(
+            self._h, C.byref(cache), batch, tokens, _ptr(first), _ptr(k_rows), _ptr(v_rows)))
+
+    def decode_kv8(self, cache: Kv8Cache, q, out, seq_lens: Sequence[int], q_heads: int,
+                   scale: Optional[float] = None) -> None:
+        scale = default_scale(cache.head_dim) if scale is None else scale
+        self._check("decode_kv8", self._lib.mslim_attn_decode_kv8(
+            self._h, C.byref(cache), _ptr(q), _ptr(out), len(seq_lens), _lens(seq_lens), q_heads, scale))
+
+    def prefill_kv8(self, cache: Kv8Cache, q, out, queries: int, priors: Sequence[int], q_heads: int,
+                    scale: Optional[float] = None) -> None:
+        """The last `queries` tokens of each sequence, already appended, over the cache."""
+        scale = default_scale(cache.head_dim) if scale is None else scale
+        self._check("prefill_kv8", self._lib.mslim_attn_prefill_kv8(
+            self._h, C.byref(cache), _ptr(q), _ptr(out), len(priors), queries, _lens(priors), q_heads, scale))
 
     def logical_kv_sha256(self, keys: Sequence, values: Sequence, tokens: int, kv_heads: int,
                           head_dim: int, page_tables: Optional[Sequence] = None,
