@@ -1275,6 +1275,30 @@ int mslim_attn_pages_gather_kv8(void *ctx, const mslim_attn_kv8_cache *cache, in
                      "8-bit gather launch");
 }
 
+// The split partials and counters of a launch, shared with the BF16 decode's.
+// Under capture nothing can be allocated: a launch whose buffers are not there
+// yet runs unsplit.
+static int kv8_workspace(Context &c, mslim::Kv8AttentionLaunch &l) {
+    const mslim::Kv8AttentionPlan plan = mslim::kv8_attention_plan(l);
+    l.split = plan.counters > 0;
+    if (!l.split) return 0;
+    if (plan.partial_bytes > c.workspace_bytes || plan.counters * sizeof(int) > c.counter_bytes) {
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        if (int rc = check_hip(hipStreamIsCapturing(c.stream, &capture), "hipStreamIsCapturing")) return rc;
+        if (capture != hipStreamCaptureStatusNone) {
+            l.split = false;
+            return 0;
+        }
+    }
+    if (int rc = grow_recorded(c, &c.workspace, &c.workspace_bytes, plan.partial_bytes,
+                               "hipMalloc decode split workspace"))
+        return rc;
+    if (int rc = split_counters(c, plan.counters)) return rc;
+    l.partial = static_cast<float *>(c.workspace);
+    l.counters = c.counters;
+    return 0;
+}
+
 // Attention over the 8-bit cache of sequences with lens[b] tokens before
 // `more` appended ones, arguments that both entry points share checked here.
 static int kv8_attention(void *ctx, const mslim_attn_kv8_cache *cache, const void *q, void *out, int batch,
@@ -1306,7 +1330,11 @@ static int kv8_attention(void *ctx, const mslim_attn_kv8_cache *cache, const voi
         l.out = static_cast<uint16_t *>(out) + b0 * row;
         l.cache.table = cache->page_table + (int64_t)b0 * cache->pages_per_seq;
         for (int b = 0; b < l.batch; ++b) l.len[b] = lens[b0 + b] + more;
-        if (int rc = check_hip(mslim::launch_kv8_attention(l, c.stream), "8-bit attention launch")) return rc;
+        if (int rc = kv8_workspace(c, l)) return rc;
+        if (int rc = check_hip(mslim::launch_kv8_attention(l, c.stream), "8-bit attention launch")) {
+            if (l.split) c.counters_dirty = true;
+            return rc;
+        }
     }
     return 0;
 }

@@ -185,6 +185,18 @@ __device__ __forceinline__ float half_pair_max(float x) {
 __device__ __forceinline__ void pin_value(uint32_t &x) { asm volatile("" : "+v"(x)); }
 __device__ __forceinline__ void pin_value(float &x) { asm volatile("" : "+v"(x)); }
 
+// Relaxed agent-scope atomics on float pairs (8-byte aligned): coherent
+// across the XCDs' L2 caches.
+__device__ __forceinline__ void store_coherent2(float *p, float x, float y) {
+    const uint64_t w = (uint64_t)__float_as_uint(x) | ((uint64_t)__float_as_uint(y) << 32);
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_coherent2(const float *p) {
+    const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32)));
+}
+
 // Butterfly reductions across the 64-lane wavefront.
 __device__ __forceinline__ float wave_xor_max(float v, int mask) {
     return fmaxf(v, __shfl_xor(v, mask, 64));

@@ -384,24 +384,56 @@ __global__ __launch_bounds__(256) void gather_kernel(Kv8Cache c, int batch, int 
 // ---- attention ---------------------------------------------------------------
 
 constexpr int kWaves = 4;
-constexpr int kTile = 32;  // tokens of a wavefront's step: two blocks
-constexpr int kRows = 16;  // query rows of a workgroup: one MFMA tile
+constexpr int kTile = 32;                // tokens of a wavefront's step: two blocks
+constexpr int kChunk = kWaves * kTile;   // tokens of a workgroup's step
+constexpr int kCus = 256;
 
 struct AttentionArgs {
     Kv8Cache cache;
     const uint16_t *q;
     uint16_t *out;
+    float *partial;  // [2 * workgroups][rows of a tile][head_dim + 2]: the accumulators, then (m, l)
+    int *counters;   // [batch][kv_heads * row_tiles] parts done, zero between launches
     int batch, queries, q_heads;
-    int row_tiles;  // of a kv head's queries * group rows
+    int row_tiles;   // of a kv head's queries * group rows
     float scale_log2e;
+    // Segments (sequence, kv head, row tile) have as many chunks as their
+    // sequence.  Workgroup w of a split launch takes the chunks w * total /
+    // workgroups .. of all segments laid end to end, so all get the same work
+    // whatever the lengths; an unsplit launch has a workgroup per segment.
+    bool split;
+    int64_t total, workgroups;
+    int64_t begin[kKv8Batch + 1];  // first chunk of each sequence
     int len[kKv8Batch];
 };
 
-// A workgroup of four wavefronts takes 16 query rows of one kv head ((query,
-// head of the group) pairs) over all their tokens, the wavefronts 32 tokens
-// each in turn:
+__host__ __device__ inline int chunks_of(int len) { return len > 0 ? (len + kChunk - 1) / kChunk : 1; }
+
+// Loads of a wavefront's step: K row pieces, V pieces and the two scales of
+// both blocks.
+template <int KP>
+struct TileRegs {
+    u32x4_t k[2][KP], v[2][KP];
+    float2 scale[2];
+};
+
+// Four outputs of a row with the sum l; one that sees nothing is zeros.
+__device__ __forceinline__ void write_row(uint16_t *out, const float4 &o, float l) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint2 packed;
+    packed.x = pack_bf16x2(o.x * inv, o.y * inv);
+    packed.y = pack_bf16x2(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2 *>(out) = packed;
+}
+
+// A workgroup of four wavefronts takes 16 * NT query rows of one kv head
+// ((query, head of the group) pairs) over a run of 128-token chunks, the
+// wavefronts 32 tokens each of a chunk:
+//   * K and V are an HBM stream: each wavefront keeps a ring of DEPTH steps
+//     in registers, DEPTH - 1 of them in flight while one is computed, and
+//     reads the page numbers of a step one step before its loads go out;
 //   * S^T = K.Q^T on v_mfma_f32_16x16x32_bf16, 16 tokens of a block as M and
-//     the rows as N.  A lane's 16 bytes of a K row widen to the A operands of
+//     16 rows as N.  A lane's 16 bytes of a K row widen to the A operands of
 //     two MFMAs, whose 8 dims per lane group are taken from Q in that order;
 //   * the scores take the block's K scale times scale * log2(e) in f32;
 //   * P goes to the P.V MFMA from the accumulator where S^T left it, in BF16
@@ -409,174 +441,342 @@ struct AttentionArgs {
 //     the rounded P, so O / l is a convex combination of V rows;
 //   * a lane's 16 bytes of V are four dims of four tokens: the B operand's
 //     tokens of its lane group;
-//   * the four wavefronts merge in LDS.
+//   * the four wavefronts merge in LDS, the parts of a segment that several
+//     workgroups took in the one that ends last, in the order of the tokens.
 // DM: head_dim rounded up to 64, 128 or 256; FULL: equal to it.
-template <int FMT, int DM, bool FULL>
-__global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionArgs a) {
+template <int FMT, int DM, bool FULL, int NT, int DEPTH, int WGS>
+__global__ __launch_bounds__(64 * kWaves, WGS) void attention_kernel(AttentionArgs a) {
     constexpr int KP = DM / 64;  // 16-byte pieces of a lane per block
-    __shared__ float comb_ml[kWaves][kRows][2];
-    __shared__ __align__(16) float comb_acc[kWaves][kRows][DM];
+    constexpr int ROWS = 16 * NT;
+    __shared__ float comb_ml[kWaves][ROWS][2];
+    __shared__ __align__(16) float comb_acc[kWaves][16][DM];
+    __shared__ int last_part;
     const Kv8Cache &c = a.cache;
     const int d = FULL ? DM : c.head_dim;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int row16 = lane & 15, grp = lane >> 4;
     const int group = a.q_heads / c.kv_heads;
-    const int rt = (int)(blockIdx.x % a.row_tiles);
-    const int head = (int)(blockIdx.x / a.row_tiles % c.kv_heads);
-    const int b = (int)(blockIdx.x / a.row_tiles / c.kv_heads);
-    const int len = a.len[b];
     const int rows = a.queries * group;
+    const int segments = c.kv_heads * a.row_tiles;  // of a sequence
 
-    // Row r of a kv head is (query r / group, head r % group of the group).
-    auto row_at = [&](int r) {
-        return (((int64_t)b * a.queries + r / group) * a.q_heads + head * group + r % group) * d;
-    };
-    const int my_row = rt * kRows + row16;
-    const int first_limit = len - a.queries + rt * kRows / group + 1;  // tokens that the tile's first row sees
-    const int limit = my_row < rows ? len - a.queries + my_row / group + 1 : 0;
-    bf16x8_t qf[KP][2];
+    // Chunks [ch, ch_end) of segment `seg` of sequence b.
+    auto run = [&](int b, int seg, int ch, int ch_end) __attribute__((always_inline)) {
+        const int head = seg / a.row_tiles, rt = seg % a.row_tiles;
+        const int len = a.len[b], nch = chunks_of(len);
+        // Row r of a kv head is (query r / group, head r % group of the group).
+        auto row_at = [&](int r) {
+            return (((int64_t)b * a.queries + r / group) * a.q_heads + head * group + r % group) * d;
+        };
+        const int first_limit = len - a.queries + rt * ROWS / group + 1;  // tokens that the tile's first row sees
+        int limit[NT];
+        bf16x8_t qf[NT][KP][2];
 #pragma unroll
-    for (int j = 0; j < KP; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int at = j * 64 + grp * 16 + h * 8;
-            qf[j][h] = bf16x8_t{};
-            if (my_row < rows && (FULL || at < d))
-                qf[j][h] = *reinterpret_cast<const bf16x8_t *>(a.q + row_at(my_row) + at);
-        }
-
-    float m_run = -__FLT_MAX__, l_run = 0.0f;
-    floatx4_t o[KP * 4];  // O[row 4*grp+i][dim 64*(sl/4) + 4*row16 + sl%4]
-#pragma unroll
-    for (int sl = 0; sl < KP * 4; ++sl) o[sl] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
-
-    for (int t0 = wave * kTile; t0 < len; t0 += kWaves * kTile) {
-        u32x4_t k[2][KP], v[2][KP];
-        float2 sc[2];
-        bool whole = t0 + kTile <= first_limit;
-        int tokens[2];  // of a block that any row may see
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-            const int bt = t0 + blk * 16;
-            const int64_t block = bt < len ? block_of(c, b, head, bt) : -1;
-            tokens[blk] = block >= 0 ? min(16, len - bt) : 0;
-            whole &= block >= 0;
-            const int64_t at = max(block, (int64_t)0);
-            sc[blk] = reinterpret_cast<const float2 *>(c.scales)[at];
-            const uint8_t *kb = c.k + at * 16 * d + row16 * d + grp * 16;
-            const uint8_t *vb = c.v + at * 16 * d + grp * d * 4 + row16 * 16;
-#pragma unroll
-            for (int j = 0; j < KP; ++j) {
-                k[blk][j] = v[blk][j] = u32x4_t{0, 0, 0, 0};
-                if (FULL || j * 64 + grp * 16 < d) k[blk][j] = *reinterpret_cast<const u32x4_t *>(kb + j * 64);
-                if (FULL || j * 64 + row16 * 4 < d) v[blk][j] = *reinterpret_cast<const u32x4_t *>(vb + j * 256);
-            }
-        }
-        floatx4_t s[2];
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-            s[blk] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < NT; ++t) {
+            const int r = rt * ROWS + t * 16 + row16;
+            limit[t] = r < rows ? len - a.queries + r / group + 1 : 0;
 #pragma unroll
             for (int j = 0; j < KP; ++j)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    s[blk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        widen8<FMT>(k[blk][j][2 * h], k[blk][j][2 * h + 1]), qf[j][h], s[blk], 0, 0, 0);
-            const float ks = sc[blk].x * a.scale_log2e;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[blk][i] *= ks;
+                for (int h = 0; h < 2; ++h) {
+                    const int at = j * 64 + grp * 16 + h * 8;
+                    qf[t][j][h] = bf16x8_t{};
+                    if (r < rows && (FULL || at < d))
+                        qf[t][j][h] = *reinterpret_cast<const bf16x8_t *>(a.q + row_at(r) + at);
+                }
         }
-        // Tokens that a row does not see weigh nothing, whatever their bytes
-        // and scales hold.
-        if (!whole) {
+
+        // Loads never branch: a block past the end repeats the last one, an
+        // entry that names no page reads page 0, a piece past head_dim the
+        // row's last one; what they bring is masked below.
+        const int t_first = ch * kChunk + wave * kTile, t_end = min(len, ch_end * kChunk);
+        const int32_t *table = c.table + (int64_t)b * c.pages_per_seq;
+        const int last = max(len - 1, 0) & ~15;
+        const int in_page = (1 << c.shift) - 1;
+        struct Pages {
+            int p[2];
+        };
+        auto pages_at = [&](int t0) {
+            return Pages{{table[min(t0, last) >> c.shift], table[min(t0 + 16, last) >> c.shift]}};
+        };
+        auto known = [&](int page) { return page >= 0 && page < (int)c.pool_pages; };
+        const int k_at = row16 * d + grp * 16, v_at = grp * d * 4 + row16 * 16;
+        auto load_tile = [&](TileRegs<KP> &r, Pages pg, int t0) {
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
-                const int at = t0 + blk * 16 + grp * 4;
-                const int fill = min(max(tokens[blk] - grp * 4, 0), 4);
-                const uint32_t keep = fill == 4 ? 0xffffffffu : (1u << (8 * fill)) - 1;
+                const int bt = min(t0 + blk * 16, last);
+                const int64_t page = known(pg.p[blk]) ? pg.p[blk] : 0;
+                const int64_t block = ((page * c.kv_heads + head) << (c.shift - 4)) + ((bt & in_page) >> 4);
+                r.scale[blk] = reinterpret_cast<const float2 *>(c.scales)[block];
+                const uint8_t *kb = c.k + block * 16 * d, *vb = c.v + block * 16 * d;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i >= fill || at + i >= limit) s[blk][i] = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < KP; ++j) v[blk][j] &= keep;
+                for (int j = 0; j < KP; ++j) {
+                    r.k[blk][j] = *reinterpret_cast<const u32x4_t *>(
+                        kb + (FULL ? k_at + j * 64 : row16 * d + min(j * 64 + grp * 16, d - 16)));
+                    r.v[blk][j] = *reinterpret_cast<const u32x4_t *>(
+                        vb + (FULL ? v_at + j * 256 : grp * d * 4 + min(j * 64 + row16 * 4, d - 4) * 4));
+                }
             }
-        }
-        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                         fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        mx = wave_xor_max(mx, 16);
-        mx = wave_xor_max(mx, 32);
-        const float m_new = fmaxf(m_run, mx);
-        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-        bf16x8_t p;
-        float psum = 0.0f;
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float pr = round_bf16(__builtin_amdgcn_exp2f(s[blk][i] - m_new));
-                psum += pr;
-                // a NaN scale of tokens that the row does not see stays out
-                p[blk * 4 + i] = (__bf16)(s[blk][i] == -INFINITY ? 0.0f : pr * sc[blk].y);
-            }
-        l_run = l_run * alpha + psum;
-        m_run = m_new;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float ai = __shfl(alpha, 4 * grp + i, 64);
-#pragma unroll
-            for (int sl = 0; sl < KP * 4; ++sl) o[sl][i] *= ai;
-        }
-#pragma unroll
-        for (int sl = 0; sl < KP * 4; ++sl)
-            o[sl] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p, widen8<FMT>(v[0][sl / 4][sl % 4], v[1][sl / 4][sl % 4]),
-                                                            o[sl], 0, 0, 0);
-    }
+        };
 
-    l_run = wave_xor_sum(l_run, 16);
-    l_run = wave_xor_sum(l_run, 32);
+        float m_run[NT], l_run[NT];
+        floatx4_t o[NT][KP * 4];  // O[row 4*grp+i][dim 64*(sl/4) + 4*row16 + sl%4]
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int t = 0; t < NT; ++t) {
+            m_run[t] = -__FLT_MAX__;
+            l_run[t] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < KP; ++j)
-            *reinterpret_cast<float4 *>(&comb_acc[wave][4 * grp + i][j * 64 + row16 * 4]) =
-                make_float4(o[j * 4][i], o[j * 4 + 1][i], o[j * 4 + 2][i], o[j * 4 + 3][i]);
-    if (lane < kRows) {
-        comb_ml[wave][lane][0] = m_run;
-        comb_ml[wave][lane][1] = l_run;
-    }
-    __syncthreads();
-    const int here = min(kRows, rows - rt * kRows);
-    for (int it = tid; it < here * (d / 4); it += 64 * kWaves) {
-        const int r = it / (d / 4), at = it % (d / 4) * 4;
-        float m = -__FLT_MAX__;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, comb_ml[w][r][0]);
-        float l = 0.0f;
-        float4 ov = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float wt = __builtin_amdgcn_exp2f(comb_ml[w][r][0] - m);
-            l = fmaf(comb_ml[w][r][1], wt, l);
-            const float4 y = *reinterpret_cast<const float4 *>(&comb_acc[w][r][at]);
-            ov.x = fmaf(y.x, wt, ov.x); ov.y = fmaf(y.y, wt, ov.y);
-            ov.z = fmaf(y.z, wt, ov.z); ov.w = fmaf(y.w, wt, ov.w);
+            for (int sl = 0; sl < KP * 4; ++sl) o[t][sl] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        // a row that sees nothing is zeros
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint2 packed;
-        packed.x = pack_bf16x2(ov.x * inv, ov.y * inv);
-        packed.y = pack_bf16x2(ov.z * inv, ov.w * inv);
-        *reinterpret_cast<uint2 *>(a.out + row_at(rt * kRows + r) + at) = packed;
+
+        auto compute_tile = [&](TileRegs<KP> &r, Pages pg, int t0) {
+            floatx4_t s[NT][2];
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) s[t][blk] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < KP; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        bf16x8_t kf = widen8<FMT>(r.k[blk][j][2 * h], r.k[blk][j][2 * h + 1]);
+                        if (!FULL && j * 64 + grp * 16 >= d) kf = bf16x8_t{};
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+                            s[t][blk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][j][h], s[t][blk], 0, 0, 0);
+                    }
+                const float ks = r.scale[blk].x * a.scale_log2e;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[t][blk][i] *= ks;
+            }
+            // Tokens that a row does not see weigh nothing, whatever their
+            // bytes and scales hold.
+            if (t0 + kTile > first_limit || !known(pg.p[0]) || !known(pg.p[1])) {
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk) {
+                    const int at = t0 + blk * 16 + grp * 4;
+                    const int fill = known(pg.p[blk]) ? min(max(len - at, 0), 4) : 0;
+                    const uint32_t keep = fill == 4 ? 0xffffffffu : (1u << (8 * fill)) - 1;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (i >= fill || at + i >= limit[t]) s[t][blk][i] = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < KP; ++j) r.v[blk][j] &= keep;
+                }
+            }
+            bf16x8_t p[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float mx = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
+                                 fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
+                mx = wave_xor_max(mx, 16);
+                mx = wave_xor_max(mx, 32);
+                const float m_new = fmaxf(m_run[t], mx);
+                if (wave_any(m_new > m_run[t])) {
+                    const float alpha = __builtin_amdgcn_exp2f(m_run[t] - m_new);
+                    l_run[t] *= alpha;
+                    m_run[t] = m_new;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float ai = __shfl(alpha, 4 * grp + i, 64);
+#pragma unroll
+                        for (int sl = 0; sl < KP * 4; ++sl) o[t][sl][i] *= ai;
+                    }
+                }
+                float psum = 0.0f;
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = s[t][blk][i];
+                        const float pr = round_bf16(__builtin_amdgcn_exp2f(x - m_run[t]));
+                        psum += pr;
+                        // a NaN scale of tokens that the row does not see stays out
+                        p[t][blk * 4 + i] = (__bf16)(x == -INFINITY ? 0.0f : pr * r.scale[blk].y);
+                    }
+                l_run[t] += psum;
+            }
+#pragma unroll
+            for (int sl = 0; sl < KP * 4; ++sl) {
+                const bf16x8_t vf = widen8<FMT>(r.v[0][sl / 4][sl % 4], r.v[1][sl / 4][sl % 4]);
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    o[t][sl] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p[t], vf, o[t][sl], 0, 0, 0);
+            }
+        };
+
+        // Ring over this wavefront's steps; past the last one the loads
+        // repeat it, so every turn issues the same ones.
+        if (t_first < t_end) {
+            const int t_last = t_first + (t_end - 1 - t_first) / kChunk * kChunk;
+            auto step_at = [&](int i) { return min(t_first + i * kChunk, t_last); };
+            TileRegs<KP> ring[DEPTH];
+            Pages pages[DEPTH + 1];
+#pragma unroll
+            for (int i = 0; i < DEPTH; ++i) pages[i] = pages_at(step_at(i));
+#pragma unroll
+            for (int i = 0; i < DEPTH - 1; ++i) load_tile(ring[i], pages[i], step_at(i));
+            for (int base = 0; t_first + base * kChunk < t_end; base += DEPTH) {
+#pragma unroll
+                for (int i = 0; i < DEPTH; ++i) {
+                    const int t0 = t_first + (base + i) * kChunk;
+                    if (t0 >= t_end) break;
+                    pages[DEPTH] = pages_at(step_at(base + i + DEPTH));
+                    load_tile(ring[(i + DEPTH - 1) % DEPTH], pages[DEPTH - 1], step_at(base + i + DEPTH - 1));
+                    __builtin_amdgcn_sched_barrier(0);
+                    compute_tile(ring[i], pages[0], t0);
+#pragma unroll
+                    for (int k = 0; k < DEPTH; ++k) pages[k] = pages[k + 1];
+                }
+            }
+        }
+
+        const bool alone = ch == 0 && ch_end == nch;
+        const int64_t seg_begin = a.begin[b] + (int64_t)seg * nch;
+        const int here = min(ROWS, rows - rt * ROWS);
+        // Slot of a workgroup's part: its last segment, which others go on
+        // with, or its first, which others have begun.
+        const int64_t slot_floats = (int64_t)ROWS * (d + 2);
+        auto part = [&](int64_t w, bool begins) { return a.partial + (2 * w + (begins ? 1 : 0)) * slot_floats; };
+        auto owner = [&](int64_t chunk) { return ((chunk + 1) * a.workgroups - 1) / a.total; };
+        float *mine = a.split ? part(owner(seg_begin + ch), ch == 0) : nullptr;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float l = wave_xor_sum(l_run[t], 16);
+            l = wave_xor_sum(l, 32);
+            if (t) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < KP; ++j)
+                    *reinterpret_cast<float4 *>(&comb_acc[wave][4 * grp + i][j * 64 + row16 * 4]) = make_float4(
+                        o[t][j * 4][i], o[t][j * 4 + 1][i], o[t][j * 4 + 2][i], o[t][j * 4 + 3][i]);
+            if (lane < 16) {
+                comb_ml[wave][t * 16 + lane][0] = m_run[t];
+                comb_ml[wave][t * 16 + lane][1] = l;
+            }
+            __syncthreads();
+            for (int it = tid; it < min(16, here - t * 16) * (d / 4); it += 64 * kWaves) {
+                const int r = it / (d / 4), at = it % (d / 4) * 4;
+                float m = -__FLT_MAX__;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) m = fmaxf(m, comb_ml[w][t * 16 + r][0]);
+                float lr = 0.0f;
+                float4 ov = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    const float wt = __builtin_amdgcn_exp2f(comb_ml[w][t * 16 + r][0] - m);
+                    lr = fmaf(comb_ml[w][t * 16 + r][1], wt, lr);
+                    const float4 y = *reinterpret_cast<const float4 *>(&comb_acc[w][r][at]);
+                    ov.x = fmaf(y.x, wt, ov.x); ov.y = fmaf(y.y, wt, ov.y);
+                    ov.z = fmaf(y.z, wt, ov.z); ov.w = fmaf(y.w, wt, ov.w);
+                }
+                if (alone) {
+                    write_row(a.out + row_at(rt * ROWS + t * 16 + r) + at, ov, lr);
+                } else {
+                    float *to = mine + (t * 16 + r) * d + at;
+                    store_coherent2(to, ov.x, ov.y);
+                    store_coherent2(to + 2, ov.z, ov.w);
+                    if (at == 0) store_coherent2(mine + ROWS * d + (t * 16 + r) * 2, m, lr);
+                }
+            }
+        }
+        if (alone) return;
+        // The parts are ordered as the BF16 decode's are: written through to
+        // the device, complete before the barrier, counted, and read past the
+        // XCD's own L2 by the workgroup that counts the last.
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        const int64_t w0 = owner(seg_begin), w1 = owner(seg_begin + nch - 1);
+        if (tid == 0) {
+            int *counter = a.counters + (int64_t)b * segments + seg;
+            const int done = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last_part = done == (int)(w1 - w0);
+            if (last_part) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!last_part) return;
+        for (int it = tid; it < here * (d / 4); it += 64 * kWaves) {
+            const int r = it / (d / 4), at = it % (d / 4) * 4;
+            float m = -__FLT_MAX__, l = 0.0f;
+            float4 ov = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            constexpr int K = 8;  // parts whose loads go out together
+            for (int64_t w = w0; w <= w1; w += K) {
+                float2 ml[K], x0[K], x1[K];
+#pragma unroll
+                for (int j = 0; j < K; ++j) {
+                    const int64_t from = min(w + j, w1);
+                    const float *src = part(from, from == w0);
+                    ml[j] = load_coherent2(src + ROWS * d + r * 2);
+                    x0[j] = load_coherent2(src + r * d + at);
+                    x1[j] = load_coherent2(src + r * d + at + 2);
+                }
+#pragma unroll
+                for (int j = 0; j < K; ++j) {
+                    if (w + j > w1) continue;
+                    const float m_new = fmaxf(m, ml[j].x);
+                    const float wo = __builtin_amdgcn_exp2f(m - m_new), wn = __builtin_amdgcn_exp2f(ml[j].x - m_new);
+                    l = fmaf(l, wo, ml[j].y * wn);
+                    ov.x = fmaf(ov.x, wo, x0[j].x * wn); ov.y = fmaf(ov.y, wo, x0[j].y * wn);
+                    ov.z = fmaf(ov.z, wo, x1[j].x * wn); ov.w = fmaf(ov.w, wo, x1[j].y * wn);
+                    m = m_new;
+                }
+            }
+            write_row(a.out + row_at(rt * ROWS + r) + at, ov, l);
+        }
+    };
+
+    if (!a.split) {
+        const int b = (int)(blockIdx.x / segments);
+        run(b, (int)(blockIdx.x % segments), 0, chunks_of(a.len[b]));
+        return;
+    }
+    int64_t at = blockIdx.x * a.total / a.workgroups;
+    const int64_t end = (blockIdx.x + 1) * a.total / a.workgroups;
+    for (bool again = false; at < end; again = true) {
+        if (again) __syncthreads();  // the LDS of the part before is free
+        int b = 0;
+        for (int hi = a.batch - 1; b < hi;) {
+            const int mid = (b + hi + 1) >> 1;
+            if (a.begin[mid] <= at) b = mid;
+            else hi = mid - 1;
+        }
+        const int nch = chunks_of(a.len[b]);
+        const int64_t local = at - a.begin[b];
+        const int seg = (int)(local / nch), ch = (int)(local % nch);
+        const int ch_end = (int)min((int64_t)nch, ch + end - at);
+        run(b, seg, ch, ch_end);
+        at += ch_end - ch;
     }
 }
 
+// Tiles of 16 rows that a launch's workgroups take together: K and V are read
+// and widened once for all of them.
+int row_tiles_at_once(const Kv8AttentionLaunch &l) {
+    const int64_t rows = (int64_t)l.queries * (l.q_heads / l.cache.kv_heads);
+    if (rows <= 16) return 1;
+    return rows <= 32 || l.cache.head_dim > 128 ? 2 : 4;
+}
+
+template <int FMT, int DM, bool FULL>
+void launch_attention(const AttentionArgs &a, int nt, unsigned grid, hipStream_t stream) {
+    const dim3 block(64 * kWaves);
+    if (nt == 1)
+        hipLaunchKernelGGL((attention_kernel<FMT, DM, FULL, 1, (DM > 128 ? 2 : 3), (DM > 128 ? 1 : 2)>), dim3(grid), block, 0, stream, a);
+    else if (nt == 2)
+        hipLaunchKernelGGL((attention_kernel<FMT, DM, FULL, 2, 2, 1>), dim3(grid), block, 0, stream, a);
+    else if constexpr (DM <= 128)
+        hipLaunchKernelGGL((attention_kernel<FMT, DM, FULL, 4, 2, 1>), dim3(grid), block, 0, stream, a);
+}
+
 template <int FMT, int DM>
-void launch_attention(const AttentionArgs &a, unsigned grid, hipStream_t stream) {
-    if (a.cache.head_dim == DM)
-        hipLaunchKernelGGL((attention_kernel<FMT, DM, true>), dim3(grid), dim3(64 * kWaves), 0, stream, a);
-    else
-        hipLaunchKernelGGL((attention_kernel<FMT, DM, false>), dim3(grid), dim3(64 * kWaves), 0, stream, a);
+void launch_attention(const AttentionArgs &a, int nt, unsigned grid, hipStream_t stream) {
+    if (a.cache.head_dim == DM) launch_attention<FMT, DM, true>(a, nt, grid, stream);
+    else launch_attention<FMT, DM, false>(a, nt, grid, stream);
 }
 
 template <int FMT>
@@ -634,21 +834,57 @@ hipError_t launch_kv8_gather(const Kv8Cache &cache, int batch, int tokens, const
     return hipGetLastError();
 }
 
+namespace {
+struct Shape {
+    int nt, row_tiles;
+    int64_t segments, total, workgroups;
+};
+// Two workgroups per CU share the chunks of all segments evenly, fewer where
+// there are fewer chunks.
+Shape shape_of(const Kv8AttentionLaunch &l) {
+    Shape s;
+    s.nt = row_tiles_at_once(l);
+    const int64_t rows = (int64_t)l.queries * (l.q_heads / l.cache.kv_heads);
+    s.row_tiles = (int)((rows + 16 * s.nt - 1) / (16 * s.nt));
+    s.segments = (int64_t)l.cache.kv_heads * s.row_tiles;
+    s.total = 0;
+    for (int b = 0; b < l.batch; ++b) s.total += chunks_of(l.len[b]) * s.segments;
+    s.workgroups = std::min<int64_t>(s.total, (s.nt == 1 && l.cache.head_dim <= 128 ? 2 : 1) * kCus);
+    return s;
+}
+}  // namespace
+
+Kv8AttentionPlan kv8_attention_plan(const Kv8AttentionLaunch &l) {
+    const Shape s = shape_of(l);
+    Kv8AttentionPlan p{};
+    if (s.segments * l.batch > 4 * s.workgroups) return p;  // as even without: nothing to merge
+    p.partial_bytes = (size_t)(2 * s.workgroups) * 16 * s.nt * (l.cache.head_dim + 2) * sizeof(float);
+    p.counters = (size_t)(s.segments * l.batch);
+    return p;
+}
+
 hipError_t launch_kv8_attention(const Kv8AttentionLaunch &l, hipStream_t stream) {
+    const Shape shape = shape_of(l);
     AttentionArgs a{};
     a.cache = l.cache;
     a.q = l.q; a.out = l.out;
+    a.partial = l.partial; a.counters = l.counters;
     a.batch = l.batch; a.queries = l.queries; a.q_heads = l.q_heads;
-    const int64_t rows = (int64_t)l.queries * (l.q_heads / l.cache.kv_heads);
-    a.row_tiles = (int)((rows + kRows - 1) / kRows);
+    a.row_tiles = shape.row_tiles;
     a.scale_log2e = l.scale * kLog2e;
-    for (int b = 0; b < l.batch; ++b) a.len[b] = l.len[b];
-    const unsigned grid = (unsigned)((int64_t)l.batch * l.cache.kv_heads * a.row_tiles);
+    a.split = l.split;
+    a.total = shape.total;
+    a.workgroups = shape.workgroups;
+    for (int b = 0; b < l.batch; ++b) {
+        a.len[b] = l.len[b];
+        a.begin[b + 1] = a.begin[b] + chunks_of(l.len[b]) * shape.segments;
+    }
+    const unsigned grid = (unsigned)(l.split ? shape.workgroups : shape.segments * l.batch);
     const int d = l.cache.head_dim;
-#define MSLIM_KV8_ATTENTION(FMT)                                        \
-    if (d <= 64) launch_attention<FMT, 64>(a, grid, stream);            \
-    else if (d <= 128) launch_attention<FMT, 128>(a, grid, stream);     \
-    else launch_attention<FMT, 256>(a, grid, stream)
+#define MSLIM_KV8_ATTENTION(FMT)                                              \
+    if (d <= 64) launch_attention<FMT, 64>(a, shape.nt, grid, stream);        \
+    else if (d <= 128) launch_attention<FMT, 128>(a, shape.nt, grid, stream); \
+    else launch_attention<FMT, 256>(a, shape.nt, grid, stream)
     if (l.cache.format == kFormatE4m3) { MSLIM_KV8_ATTENTION(kFormatE4m3); }
     else { MSLIM_KV8_ATTENTION(kFormatInt8); }
 #undef MSLIM_KV8_ATTENTION
