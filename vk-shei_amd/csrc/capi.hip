@@ -1279,7 +1279,8 @@ int mslim_attn_pages_gather_kv8(void *ctx, const mslim_attn_kv8_cache *cache, in
 // Under capture nothing can be allocated: a launch whose buffers are not there
 // yet runs unsplit.
 static int kv8_workspace(Context &c, mslim::Kv8AttentionLaunch &l) {
-    const mslim::Kv8AttentionPlan plan = mslim::kv8_attention_plan(l);
+    const mslim::Kv8AttentionPlan plan =
+        mslim::kv8_prefill_supported(l) ? mslim::kv8_prefill_plan(l) : mslim::kv8_attention_plan(l);
     l.split = plan.counters > 0;
     if (!l.split) return 0;
     if (plan.partial_bytes > c.workspace_bytes || plan.counters * sizeof(int) > c.counter_bytes) {
@@ -1331,7 +1332,9 @@ static int kv8_attention(void *ctx, const mslim_attn_kv8_cache *cache, const voi
         l.cache.table = cache->page_table + (int64_t)b0 * cache->pages_per_seq;
         for (int b = 0; b < l.batch; ++b) l.len[b] = lens[b0 + b] + more;
         if (int rc = kv8_workspace(c, l)) return rc;
-        if (int rc = check_hip(mslim::launch_kv8_attention(l, c.stream), "8-bit attention launch")) {
+        const hipError_t err = mslim::kv8_prefill_supported(l) ? mslim::launch_kv8_prefill(l, c.stream)
+                                                                : mslim::launch_kv8_attention(l, c.stream);
+        if (int rc = check_hip(err, "8-bit attention launch")) {
             if (l.split) c.counters_dirty = true;
             return rc;
         }

@@ -395,6 +395,11 @@ struct Kv8AttentionPlan {
 };
 Kv8AttentionPlan kv8_attention_plan(const Kv8AttentionLaunch &l);
 hipError_t launch_kv8_attention(const Kv8AttentionLaunch &l, hipStream_t stream);
+// The same for many rows (csrc/kv8_prefill.hip): bound by its matrix products
+// instead of the cache's bytes.
+bool kv8_prefill_supported(const Kv8AttentionLaunch &l);
+Kv8AttentionPlan kv8_prefill_plan(const Kv8AttentionLaunch &l);
+hipError_t launch_kv8_prefill(const Kv8AttentionLaunch &l, hipStream_t stream);
 
 // Canonical head-major serialisation of one layer tensor: tokens
 // [first, first+count) of kv head `head` into out[count][head_dim]

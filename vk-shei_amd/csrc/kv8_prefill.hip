@@ -1,0 +1,597 @@
+// Attention of many query rows over the 8-bit paged K/V cache: prompt chunks.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.hpp"
+#include "kernels.hpp"
+#include "kv8.hpp"
+
+namespace mslim {
+
+namespace {
+
+constexpr int kWaves = 8;
+constexpr int kRows = 32 * kWaves;  // query rows of a workgroup at most
+constexpr int kBN = 64;             // keys of a tile: four blocks
+constexpr int kCus = 256;
+constexpr int kXcds = 8;
+// The reference maximum of a row moves only when a tile's row sum under it
+// exceeds 2^8.
+constexpr float kLazyBound = 256.0f;
+
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+struct PrefillArgs {
+    Kv8Cache cache;
+    const uint16_t *q;
+    uint16_t *out;
+    float *partial;  // [2 * workgroups][wavefront][pair][64] float pairs
+    int *counters;   // [batch][kv_heads * row_tiles] parts done, zero between launches
+    int batch, queries, q_heads;
+    int tile_queries;  // queries of a row tile: kRows / group
+    int row_tiles;
+    float scale_log2e;
+    // Segments (sequence, kv head, row tile) laid end to end; workgroup w of a
+    // split launch takes tiles w * total / workgroups .. of them, an unsplit
+    // one has a workgroup per segment.
+    bool split;
+    int64_t total, workgroups;
+    int64_t begin[kKv8Batch + 1];  // first tile of each sequence
+    int64_t head_tiles[kKv8Batch];  // tiles of one kv head of each sequence
+    int prior[kKv8Batch];
+};
+
+// Tiles of row tile rt of a sequence: up to the last key its last row sees.
+__host__ __device__ inline int tiles_of(int prior, int queries, int tile_queries, int rt) {
+    const int64_t end = prior + ((int64_t)(rt + 1) * tile_queries < queries ? (int64_t)(rt + 1) * tile_queries
+                                                                            : (int64_t)queries);
+    return (int)((end + kBN - 1) / kBN);
+}
+
+// Bytes times a scale as BF16.  A power of two, what the append writes, is
+// exact; E4M3 takes it in the conversion.
+template <int FMT>
+__device__ __forceinline__ void widen_scaled(const u32x4_t &w, float scale, uint4 (&out)[2]) {
+    uint32_t o[8];
+    if (FMT == kFormatE4m3 && (__float_as_uint(scale) & 0x7fffffu) == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, false));
+            o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, true));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o[2 * i] = pack_bf16x2(byte_value<FMT>(w[i], 0) * scale, byte_value<FMT>(w[i], 1) * scale);
+            o[2 * i + 1] = pack_bf16x2(byte_value<FMT>(w[i], 2) * scale, byte_value<FMT>(w[i], 3) * scale);
+        }
+    }
+    out[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+// A workgroup of eight wavefronts takes the rows of tile_queries queries and
+// all heads of one kv head's group (32 rows per wavefront) over a run of
+// 64-key tiles:
+//   * a tile's bytes come in registers, 16 of K and 16 of V per lane, go out
+//     to LDS as BF16 once for all rows, times their block's scale (exact: a
+//     power of two), one tile ahead of use, and the loads one tile ahead of
+//     that;
+//   * S^T = K.Q^T on v_mfma_f32_32x32x16_bf16 (keys as M, a wavefront's rows
+//     as N).  The accumulator has one row per lane, in the operand layout of
+//     O^T = V^T.P^T, so P stays in registers and softmax, rescale and mask are
+//     per-lane operations;
+//   * the V^T operand's eight keys of a dim are two runs of four: the cache
+//     keeps four tokens of a dim side by side, so a fragment is two 8-byte
+//     reads without a transposition;
+//   * VALU work hides under MFMAs of the same wavefront only: the softmax of
+//     tile j runs in the slots of P.V of tile j - 1, the widening of tile
+//     j + 1 in those of Q.K of tile j;
+//   * the scores take scale * log2(e) and lose the row's reference maximum in
+//     one f32 FMA; P is rounded to BF16 for its product with V and the row
+//     sum adds the rounded P;
+//   * O is rescaled only when a tile's row sum under the reference exceeds
+//     2^8 (exact: O / l has the same reference);
+//   * a block whose scale is not finite enters as V zeros and K NaN: rows that
+//     see it get NaN, and the masked ones, whose P is zero, do not.
+template <int FMT, int DM, bool FULL>
+__global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
+    constexpr int KS = DM / 16;        // Q.K MFMA k-steps
+    constexpr int MT = DM / 32;        // P.V output tiles of 32 dims
+    constexpr int NS = 4 * MT;         // P.V MFMAs of a tile
+    constexpr int NSLOT = DM / 8;      // 16-byte slots of a K row in LDS
+    constexpr int PIECES = kBN * DM / 16;  // 16-byte pieces of a tile's K (and V) bytes: 512 or 256
+    constexpr int PAIRS = MT * 8 + 1;
+    __shared__ __align__(16) uint16_t k_lds[2][kBN * DM];
+    __shared__ __align__(16) uint16_t v_lds[3][kBN * DM];  // [block][4][dim][4 tokens]
+    __shared__ int last_part;
+
+    const Kv8Cache &c = a.cache;
+    const int d = FULL ? DM : c.head_dim;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int group = a.q_heads / c.kv_heads;
+    const float sc = a.scale_log2e;
+
+    // This lane's pieces of a tile: K piece = 16 dims of a row, V piece = 4
+    // dims of four tokens.  Both lie in one block, the same for the wavefront.
+    // DM 64: the first four wavefronts take K, the others V.
+    const bool has_k = PIECES == 512 || wave < 4, has_v = PIECES == 512 || wave >= 4;
+    const int piece = tid & (PIECES - 1);
+    const int my_block = __builtin_amdgcn_readfirstlane(PIECES == 512 ? wave >> 1 : wave & 3);
+    const int k_row = piece / (DM / 16), k_dim = piece % (DM / 16) * 16;
+    const int v_grp = piece % (DM) / (DM / 4), v_dim = piece % (DM / 4) * 4;
+    const bool k_in = FULL || k_dim < d, v_in = FULL || v_dim < d;
+    const int k_off = (k_row & 15) * d + min(k_dim, d - 16), v_off = (v_grp * d + min(v_dim, d - 4)) * 4;
+    auto k_slot = [](int row, int slot) { return slot ^ (row & (NSLOT - 1)); };
+    uint16_t *const k_to0 = &k_lds[0][k_row * DM + k_slot(k_row, k_dim / 8) * 8];
+    uint16_t *const k_to1 = &k_lds[0][k_row * DM + k_slot(k_row, k_dim / 8 + 1) * 8];
+    uint16_t *const v_to = &v_lds[0][((piece / DM * 4 + v_grp) * DM + v_dim) * 4];
+
+    // Fragment addresses in stage 0; a stage and a block of rows are immediates.
+    uint32_t k_from[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+        k_from[ks] = lds_offset(k_lds) + (uint32_t)(col * DM + k_slot(col, 2 * ks + half) * 8) * 2;
+    const uint32_t v_from = lds_offset(v_lds) + (uint32_t)(half * DM + col) * 8;
+    constexpr uint32_t STAGE = kBN * DM * 2;
+
+    auto run = [&](int b, int head, int rt, int tile, int tile_end, int64_t seg_begin, int tiles)
+        __attribute__((always_inline)) {
+        const int prior = a.prior[b];
+        const int len = prior + a.queries;
+        const int r = wave * 32 + col;  // row of the tile: (query r / group, head r % group)
+        const int query = rt * a.tile_queries + r / group;
+        const bool live = r < a.tile_queries * group && query < a.queries;
+        const int limit = live ? prior + query + 1 : 0;
+        // keys that every row of the wavefront sees
+        const int common = prior + rt * a.tile_queries + wave * 32 / group + 1;
+        const int64_t row_at =
+            (((int64_t)b * a.queries + (live ? query : 0)) * a.q_heads + head * group + r % group) * d;
+        bf16x8_t qf[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int at = ks * 16 + half * 8;
+            qf[ks] = bf16x8_t{};
+            if (live && (FULL || at < d)) qf[ks] = *reinterpret_cast<const bf16x8_t *>(a.q + row_at + at);
+        }
+
+        // Pages of a tile's four blocks; a block past the end repeats the last.
+        const int32_t *table = c.table + (int64_t)b * c.pages_per_seq;
+        const int last_block = (len - 1) & ~15;
+        struct Pages {
+            int p[4];
+        };
+        auto block_at = [&](int t, int i) { return min(t * kBN + i * 16, last_block); };
+        auto pages_at = [&](int t) {
+            Pages pg;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pg.p[i] = table[block_at(t, i) >> c.shift];
+            return pg;
+        };
+        auto known = [&](int page) { return page >= 0 && page < (int)c.pool_pages; };
+        auto all_known = [&](const Pages &pg) {
+            return known(pg.p[0]) && known(pg.p[1]) && known(pg.p[2]) && known(pg.p[3]);
+        };
+        u32x4_t k_in_regs = {}, v_in_regs = {};
+        float2 scale = make_float2(0.0f, 0.0f);
+        bool no_page = false;  // the loaded bytes are another page's
+        auto load = [&](const Pages &pg, int t) __attribute__((always_inline)) {
+            const int pick = my_block == 0 ? pg.p[0] : my_block == 1 ? pg.p[1] : my_block == 2 ? pg.p[2] : pg.p[3];
+            no_page = !known(pick);
+            const int64_t page = no_page ? 0 : pick;
+            const int64_t block = ((page * c.kv_heads + head) << (c.shift - 4)) +
+                                  ((block_at(t, my_block) & ((1 << c.shift) - 1)) >> 4);
+            scale = reinterpret_cast<const float2 *>(c.scales)[block];
+            if (has_k) k_in_regs = *reinterpret_cast<const u32x4_t *>(c.k + block * 16 * d + k_off);
+            if (has_v) v_in_regs = *reinterpret_cast<const u32x4_t *>(c.v + block * 16 * d + v_off);
+        };
+        // The loaded tile to K stage ks and V stage vs.  V bytes behind the
+        // last token, or of no page, become zeros; K's are masked.
+        auto store_k = [&](int ks) __attribute__((always_inline)) {
+            if (!has_k) return;
+            // NaN where K's or V's scale is not finite
+            const float by = (scale.y - scale.y) + scale.x;
+            uint4 w[2];
+            widen_scaled<FMT>(k_in ? k_in_regs : u32x4_t{0, 0, 0, 0}, scale.x, w);
+            if (!(__builtin_fabsf(by) <= __FLT_MAX__)) w[0] = w[1] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+            *reinterpret_cast<uint4 *>(k_to0 + ks * kBN * DM) = w[0];
+            *reinterpret_cast<uint4 *>(k_to1 + ks * kBN * DM) = w[1];
+        };
+        auto store_v = [&](int vs, int t) __attribute__((always_inline)) {
+            if (!has_v) return;
+            uint4 w[2];
+            u32x4_t bytes = v_in && !no_page ? v_in_regs : u32x4_t{0, 0, 0, 0};
+            if (t * kBN + kBN > len) {
+                const int fill = min(max(len - (t * kBN + my_block * 16 + v_grp * 4), 0), 4);
+                bytes &= fill == 4 ? 0xffffffffu : (1u << (8 * fill)) - 1;
+            }
+            widen_scaled<FMT>(bytes, scale.y, w);
+            if (!(__builtin_fabsf(scale.y) <= __FLT_MAX__)) w[0] = w[1] = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(v_to + vs * kBN * DM) = w[0];
+            *reinterpret_cast<uint4 *>(v_to + vs * kBN * DM + 8) = w[1];
+        };
+
+        floatx16_t o[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[mt][i] = 0.0f;
+        float m_used = -__FLT_MAX__, l_run = 0.0f, alpha = 1.0f;
+        bool rescale = false;
+        floatx16_t s[2];
+        bf16x8_t p[2][2];  // [key half of 32][16 of them]
+
+        // Scores of the tile in K stage st; `mid(n)` after MFMA n.
+        auto qk = [&](int st, auto &&mid) __attribute__((always_inline)) {
+            auto frag = [&](int n) __attribute__((always_inline)) {
+                return lds_read_b128(k_from[n / 2] + st * STAGE + n % 2 * 32 * DM * 2);
+            };
+            bf16x8_t kq[3];
+            kq[0] = frag(0);
+            kq[1] = frag(1);
+#pragma unroll
+            for (int n = 0; n < 2 * KS; ++n) {
+                if (n + 2 < 2 * KS) kq[(n + 2) % 3] = frag(n + 2);
+                __builtin_amdgcn_sched_barrier(0);
+                if (n < 2) {
+                    floatx16_t zero;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) zero[i] = 0.0f;
+                    s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kq[n], qf[0], zero, 0, 0, 0);
+                } else {
+                    s[n % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kq[n % 3], qf[n / 2], s[n % 2], 0, 0, 0);
+                }
+                mid(n);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // Key of element (kb, i) in its tile: kb * 32 + (i >> 2) * 8 + half * 4 + (i & 3).
+        auto mask = [&](int t, const Pages &pg) __attribute__((always_inline)) {
+            if (t * kBN + kBN > common) {
+                const int most = limit - 1 - t * kBN - half * 4;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (kb * 32 + (i >> 2) * 8 + (i & 3) > most) s[kb][i] = -INFINITY;
+            }
+            if (!all_known(pg)) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!known(pg.p[kb * 2 + i / 8])) s[kb][i] = -INFINITY;
+            }
+        };
+        auto row_max = [&]() __attribute__((always_inline)) {
+            float mx = s[0][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) mx = __builtin_fmaxf(mx, s[0][i]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, s[1][i]);
+            return half_pair_max(mx) * sc;
+        };
+        uint32_t pw[2][8];
+        float psum = 0.0f;
+        auto score_pair = [&](int n) __attribute__((always_inline)) {
+            const int kb = n / 8, i = n % 8 * 2;
+            bf16x2_t pp;
+            pp[0] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[kb][i], sc, -m_used));
+            pp[1] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[kb][i + 1], sc, -m_used));
+            pw[kb][n % 8] = __builtin_bit_cast(uint32_t, pp);
+            psum = add_bf16_pair(pp, psum);
+            pin_value(pw[kb][n % 8]);
+        };
+        // Every p is at most its tile's row sum, so the reference stays while
+        // that is within the bound; else the rows whose maximum exceeds it
+        // move it and the tile's P is taken again.
+        auto settle = [&]() __attribute__((always_inline)) {
+            if (wave_any(!(psum <= kLazyBound))) {
+                const float m_new = fmaxf(row_max(), m_used);
+                alpha = __builtin_amdgcn_exp2f(m_used - m_new);
+                l_run *= alpha;
+                m_used = m_new;
+                rescale = true;
+                psum = 0.0f;
+#pragma unroll
+                for (int n = 0; n < 16; ++n) score_pair(n);
+            }
+            l_run += psum;
+        };
+        auto keep_p = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    p[kb][t] = __builtin_bit_cast(
+                        bf16x8_t, make_uint4(pw[kb][4 * t], pw[kb][4 * t + 1], pw[kb][4 * t + 2], pw[kb][4 * t + 3]));
+        };
+        // P.V of the tile in V stage st, with the softmax of the current
+        // scores spread over its MFMAs where SOFTMAX.
+        auto pv = [&](int st, auto softmax) __attribute__((always_inline)) {
+            constexpr bool SOFTMAX = decltype(softmax)::value;
+            auto frag = [&](int n) __attribute__((always_inline)) {
+                const int mt = n % MT, t = n / MT;  // block of 16 keys
+                const uint32_t at = v_from + st * STAGE + t * 4 * DM * 8 + mt * 32 * 8;
+                const u32x2_t lo = *(const __attribute__((address_space(3))) u32x2_t *)(uintptr_t)at;
+                const u32x2_t hi = *(const __attribute__((address_space(3))) u32x2_t *)(uintptr_t)(at + 2 * DM * 8);
+                return __builtin_bit_cast(bf16x8_t, u32x4_t{lo[0], lo[1], hi[0], hi[1]});
+            };
+            if constexpr (SOFTMAX) psum = 0.0f;
+            bf16x8_t vq[3];
+            vq[0] = frag(0);
+            vq[1] = frag(1);
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                if (n + 2 < NS) vq[(n + 2) % 3] = frag(n + 2);
+                __builtin_amdgcn_sched_barrier(0);
+                o[n % MT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vq[n % 3], p[n / MT / 2][n / MT % 2], o[n % MT], 0, 0, 0);
+                if constexpr (SOFTMAX) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (k * NS / 16 == n) score_pair(k);
+                    pin_value(psum);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // All wavefronts' LDS accesses before it are done; global loads stay
+        // in flight.
+        auto barrier = [&]() __attribute__((always_inline)) {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0xF | (3 << 14) | (0x7 << 4));  // lgkmcnt 0
+            raw_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" ::: "memory");
+        };
+
+        const int last_tile = tile_end - 1;
+        auto clamp = [&](int t) { return min(t, last_tile); };
+        Pages pg0 = pages_at(tile), pg1 = pages_at(clamp(tile + 1)), pg2 = pages_at(clamp(tile + 2));
+        load(pg0, tile);
+        store_k(0);
+        store_v(0, tile);
+        load(pg1, clamp(tile + 1));
+        barrier();
+        // First tile: scores, their maximum, P.
+        qk(0, [&](int n) __attribute__((always_inline)) {
+            if (n == 3) store_k(1);
+            if (n == KS + 1) store_v(1, clamp(tile + 1));
+            if (n == 2 * KS - 2) load(pg2, clamp(tile + 2));
+        });
+        mask(tile, pg0);
+        m_used = fmaxf(row_max(), m_used);
+#pragma unroll
+        for (int n = 0; n < 16; ++n) score_pair(n);
+        l_run = psum;
+        keep_p();
+        int ks = 1, vs = 0;  // stages of K of tile j and V of tile j - 1
+        for (int j = tile + 1; j < tile_end; ++j) {
+            pg0 = pg1;
+            pg1 = pg2;
+            pg2 = pages_at(clamp(j + 2));
+            barrier();
+            if (rescale) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[mt][i] *= alpha;
+                rescale = false;
+            }
+            const int vn = vs == 0 ? 2 : vs - 1;  // of V of tile j + 1
+            qk(ks, [&](int n) __attribute__((always_inline)) {
+                if (n == 3) store_k(ks ^ 1);
+                if (n == KS + 1) store_v(vn, clamp(j + 1));
+                if (n == 2 * KS - 2) load(pg2, clamp(j + 2));
+            });
+            mask(j, pg0);
+            pv(vs, std::true_type{});
+            settle();
+            keep_p();
+            ks ^= 1;
+            vs = vs == 2 ? 0 : vs + 1;
+        }
+        if (rescale) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[mt][i] *= alpha;
+        }
+        pv(vs, std::false_type{});
+
+        float l = l_run + __shfl_xor(l_run, 32, 64);
+        auto write_out = [&](const floatx16_t *acc, float lsum) __attribute__((always_inline)) {
+            if (!live) return;
+            const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;  // a row that sees nothing is zeros
+            uint16_t *op = a.out + row_at + half * 4;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4) {
+                    uint2 w;
+                    w.x = pack_bf16x2(acc[mt][i4 * 4] * inv, acc[mt][i4 * 4 + 1] * inv);
+                    w.y = pack_bf16x2(acc[mt][i4 * 4 + 2] * inv, acc[mt][i4 * 4 + 3] * inv);
+                    if (FULL || mt * 32 + i4 * 8 < d) *reinterpret_cast<uint2 *>(op + mt * 32 + i4 * 8) = w;
+                }
+        };
+        if (tile == 0 && tile_end == tiles) {
+            write_out(o, l);
+            return;
+        }
+        // Parts of a segment: written through to the device, complete before
+        // the barrier, counted, and merged in the order of the keys by the
+        // workgroup that counts the last (as the decode's are).
+        auto owner = [&](int64_t t) { return ((t + 1) * a.workgroups - 1) / a.total; };
+        auto part = [&](int64_t w, bool begins) {
+            return a.partial + (((2 * w + (begins ? 1 : 0)) * kWaves + wave) * PAIRS * 64 + lane) * 2;
+        };
+        float *mine = part(owner(seg_begin + tile), tile == 0);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) store_coherent2(mine + (mt * 8 + i) * 128, o[mt][2 * i], o[mt][2 * i + 1]);
+        store_coherent2(mine + MT * 8 * 128, m_used, l);
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        const int64_t w0 = owner(seg_begin), w1 = owner(seg_begin + tiles - 1);
+        if (tid == 0) {
+            int *counter = a.counters + ((int64_t)b * c.kv_heads + head) * a.row_tiles + rt;
+            const int done = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last_part = done == (int)(w1 - w0);
+            if (last_part) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!last_part) return;
+        float m = -__FLT_MAX__;
+        l = 0.0f;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[mt][i] = 0.0f;
+        for (int64_t w = w0; w <= w1; ++w) {
+            const float *from = part(w, w == w0);
+            float2 x[MT * 8];
+#pragma unroll
+            for (int e = 0; e < MT * 8; ++e) x[e] = load_coherent2(from + e * 128);
+            const float2 ml = load_coherent2(from + MT * 8 * 128);
+            const float m_new = fmaxf(m, ml.x);
+            const float wo = __builtin_amdgcn_exp2f(m - m_new), wn = __builtin_amdgcn_exp2f(ml.x - m_new);
+            l = fmaf(l, wo, ml.y * wn);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    o[mt][2 * i] = fmaf(o[mt][2 * i], wo, x[mt * 8 + i].x * wn);
+                    o[mt][2 * i + 1] = fmaf(o[mt][2 * i + 1], wo, x[mt * 8 + i].y * wn);
+                }
+            m = m_new;
+        }
+        write_out(o, l);
+    };
+
+    // Workgroup -> run of tiles: XCD x (workgroups x, x + 8, ...) takes a
+    // contiguous eighth of all, so the kv heads that it reads stay in its L2.
+    int64_t at, end;
+    if (a.split) {
+        const int64_t per_xcd = a.workgroups / kXcds;
+        const int64_t w = a.workgroups % kXcds ? blockIdx.x : blockIdx.x % kXcds * per_xcd + blockIdx.x / kXcds;
+        at = w * a.total / a.workgroups;
+        end = (w + 1) * a.total / a.workgroups;
+    } else {
+        // segment blockIdx.x: found like a tile below, its run is all of it
+        const int64_t seg = blockIdx.x;
+        const int per_seq = c.kv_heads * a.row_tiles;
+        const int b = (int)(seg / per_seq), rest = (int)(seg % per_seq);
+        at = a.begin[b] + (int64_t)(rest / a.row_tiles) * a.head_tiles[b];
+        for (int rt = 0; rt < rest % a.row_tiles; ++rt) at += tiles_of(a.prior[b], a.queries, a.tile_queries, rt);
+        end = at + tiles_of(a.prior[b], a.queries, a.tile_queries, rest % a.row_tiles);
+    }
+    int b = 0;
+    for (int hi = a.batch - 1; b < hi;) {
+        const int mid = (b + hi + 1) >> 1;
+        if (a.begin[mid] <= at) b = mid;
+        else hi = mid - 1;
+    }
+    int head = (int)((at - a.begin[b]) / a.head_tiles[b]), rt = 0;
+    int64_t seg_begin = a.begin[b] + (int64_t)head * a.head_tiles[b];
+    int tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, 0);
+    while (seg_begin + tiles <= at) {
+        seg_begin += tiles;
+        tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, ++rt);
+    }
+    for (bool again = false; at < end; again = true) {
+        if (again) __syncthreads();  // the LDS of the part before is free
+        const int tile = (int)(at - seg_begin), tile_end = (int)min((int64_t)tiles, end - seg_begin);
+        run(b, head, rt, tile, tile_end, seg_begin, tiles);
+        at = seg_begin + tile_end;
+        seg_begin += tiles;
+        if (++rt == a.row_tiles) {
+            rt = 0;
+            if (++head == c.kv_heads) {
+                head = 0;
+                b = min(b + 1, a.batch - 1);
+            }
+        }
+        tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, rt);
+    }
+}
+
+struct Shape {
+    int tile_queries, row_tiles;
+    int64_t total, workgroups, segments;
+    int64_t begin[kKv8Batch + 1];
+    int64_t head_tiles[kKv8Batch];
+};
+Shape shape_of(const Kv8AttentionLaunch &l) {
+    Shape s{};
+    s.tile_queries = kRows / (l.q_heads / l.cache.kv_heads);
+    s.row_tiles = (l.queries + s.tile_queries - 1) / s.tile_queries;
+    s.segments = (int64_t)l.batch * l.cache.kv_heads * s.row_tiles;
+    for (int b = 0; b < l.batch; ++b) {
+        int64_t tiles = 0;
+        for (int rt = 0; rt < s.row_tiles; ++rt) tiles += tiles_of(l.len[b] - l.queries, l.queries, s.tile_queries, rt);
+        s.head_tiles[b] = tiles;
+        s.begin[b + 1] = s.begin[b] + tiles * l.cache.kv_heads;
+    }
+    s.total = s.begin[l.batch];
+    s.workgroups = std::min<int64_t>(s.total, kCus);
+    return s;
+}
+
+template <int FMT, int DM>
+void launch(const PrefillArgs &a, unsigned grid, hipStream_t stream) {
+    if (a.cache.head_dim == DM)
+        hipLaunchKernelGGL((kv8_prefill_kernel<FMT, DM, true>), dim3(grid), dim3(512), 0, stream, a);
+    else
+        hipLaunchKernelGGL((kv8_prefill_kernel<FMT, DM, false>), dim3(grid), dim3(512), 0, stream, a);
+}
+
+}  // namespace
+
+bool kv8_prefill_supported(const Kv8AttentionLaunch &l) {
+    const int group = l.q_heads / l.cache.kv_heads;
+    const int64_t rows = (int64_t)l.queries * group;
+    return l.cache.head_dim <= 128 && group <= kRows && rows > 64;
+}
+
+Kv8AttentionPlan kv8_prefill_plan(const Kv8AttentionLaunch &l) {
+    const Shape s = shape_of(l);
+    Kv8AttentionPlan p{};
+    const int pairs = (l.cache.head_dim <= 64 ? 2 : 4) * 8 + 1;
+    p.partial_bytes = (size_t)(2 * s.workgroups) * kWaves * pairs * 64 * 2 * sizeof(float);
+    p.counters = (size_t)s.segments;
+    return p;
+}
+
+hipError_t launch_kv8_prefill(const Kv8AttentionLaunch &l, hipStream_t stream) {
+    const Shape s = shape_of(l);
+    PrefillArgs a{};
+    a.cache = l.cache;
+    a.q = l.q; a.out = l.out;
+    a.partial = l.partial; a.counters = l.counters;
+    a.batch = l.batch; a.queries = l.queries; a.q_heads = l.q_heads;
+    a.tile_queries = s.tile_queries;
+    a.row_tiles = s.row_tiles;
+    a.scale_log2e = l.scale * kLog2e;
+    a.split = l.split;
+    a.total = s.total;
+    a.workgroups = s.workgroups;
+    for (int b = 0; b < l.batch; ++b) {
+        a.begin[b + 1] = s.begin[b + 1];
+        a.head_tiles[b] = s.head_tiles[b];
+        a.prior[b] = l.len[b] - l.queries;
+    }
+    const unsigned grid = (unsigned)(l.split ? s.workgroups : s.segments);
+#define MSLIM_KV8_PREFILL(FMT)                                              \
+    if (l.cache.head_dim <= 64) launch<FMT, 64>(a, grid, stream);           \
+    else launch<FMT, 128>(a, grid, stream)
+    if (l.cache.format == kFormatE4m3) { MSLIM_KV8_PREFILL(kFormatE4m3); }
+    else { MSLIM_KV8_PREFILL(kFormatInt8); }
+#undef MSLIM_KV8_PREFILL
+    return hipGetLastError();
+}
+
+}  // namespace mslim
