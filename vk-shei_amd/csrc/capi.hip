@@ -1281,7 +1281,7 @@ int mslim_attn_pages_gather_kv8(void *ctx, const mslim_attn_kv8_cache *cache, in
 static int kv8_workspace(Context &c, mslim::Kv8AttentionLaunch &l) {
     const mslim::Kv8AttentionPlan plan =
         mslim::kv8_prefill_supported(l) ? mslim::kv8_prefill_plan(l) : mslim::kv8_attention_plan(l);
-    l.split = plan.counters > 0;
+    l.split = plan.split;
     if (!l.split) return 0;
     if (plan.partial_bytes > c.workspace_bytes || plan.counters * sizeof(int) > c.counter_bytes) {
         hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
@@ -1294,7 +1294,8 @@ static int kv8_workspace(Context &c, mslim::Kv8AttentionLaunch &l) {
     if (int rc = grow_recorded(c, &c.workspace, &c.workspace_bytes, plan.partial_bytes,
                                "hipMalloc decode split workspace"))
         return rc;
-    if (int rc = split_counters(c, plan.counters)) return rc;
+    if (plan.counters)
+        if (int rc = split_counters(c, plan.counters)) return rc;
     l.partial = static_cast<float *>(c.workspace);
     l.counters = c.counters;
     return 0;

@@ -382,16 +382,17 @@ struct Kv8AttentionLaunch {
     int batch, queries, q_heads;
     float scale;
     int len[kKv8Batch];  // 0: nothing cached, the rows are zeros
-    // Split launches (kv8_attention_plan): partials and counters, the latter
-    // zero between launches.  Without them (split false) every workgroup takes
-    // its rows' tokens alone.
+    // Split launches (the plan's): partials and counters, the latter zero
+    // between launches.  Without them (split false) every workgroup takes its
+    // rows' tokens alone.
     bool split;
     float *partial;
     int *counters;
 };
 struct Kv8AttentionPlan {
+    bool split;
     size_t partial_bytes;
-    size_t counters;  // ints; 0: the launch does not split
+    size_t counters;  // ints
 };
 Kv8AttentionPlan kv8_attention_plan(const Kv8AttentionLaunch &l);
 hipError_t launch_kv8_attention(const Kv8AttentionLaunch &l, hipStream_t stream);

@@ -8,6 +8,8 @@
 // side ([4][head_dim][4] bytes per block): that is the order in which the P.V
 // MFMA wants its operand, so V needs no transposition through LDS.
 #include <algorithm>
+#include <climits>
+#include <type_traits>
 
 #include "common.hpp"
 #include "kernels.hpp"
@@ -347,10 +349,25 @@ __global__ __launch_bounds__(256) void gather_kernel(Kv8Cache c, int batch, int 
 
 // ---- attention ---------------------------------------------------------------
 
-constexpr int kWaves = 4;
 constexpr int kTile = 32;                // tokens of a wavefront's step: two blocks
-constexpr int kChunk = kWaves * kTile;   // tokens of a workgroup's step
 constexpr int kCus = 256;
+constexpr int kMergeParts = 16;          // parts that a merging thread loads at once
+// Calls that read more than the Infinity Cache holds load K and V
+// non-temporally: 538 MB 99.8 -> 92.0 us, 269 MB 53.2 -> 51.0 us, 67 MB
+// 20.0 -> 22.1 us.
+constexpr int64_t kStreamBytes = 200ll << 20;
+// A segment's parts above these bytes merge in a launch of their own, a
+// workgroup per row, instead of in the workgroup that ends last, to which the
+// device's memory gives about 25 GB/s: eight rows of four heads after 8,000
+// tokens, 530 KB a segment, 35.3 -> 19.7 us; at 66 KB (one row of four heads)
+// 13.5 and 12.3 us, at 33 KB equal.
+constexpr int64_t kMergeLaunchBytes = 64 << 10;
+// Workgroups of eight wavefronts, one per CU, instead of four, two per CU,
+// where segments have at least this many parts: half as many to merge (8,192
+// tokens, 64 parts: 19.8 -> 13.5 us; 4 x 32,768 56.5 -> 53.2 us).  With
+// several segments to a workgroup the switch from one to the next stalls
+// twice the wavefronts: 32 sequences of 512 .. 8,192 tokens 63 -> 68 us.
+constexpr int kWideParts = 12;
 
 struct AttentionArgs {
     Kv8Cache cache;
@@ -362,16 +379,27 @@ struct AttentionArgs {
     int row_tiles;   // of a kv head's queries * group rows
     float scale_log2e;
     // Segments (sequence, kv head, row tile) have as many chunks as their
-    // sequence.  Workgroup w of a split launch takes the chunks w * total /
-    // workgroups .. of all segments laid end to end, so all get the same work
-    // whatever the lengths; an unsplit launch has a workgroup per segment.
-    bool split;
-    int64_t total, workgroups;
-    int64_t begin[kKv8Batch + 1];  // first chunk of each sequence
+    // sequence.  Laid end to end, workgroup w of a split launch takes `share`
+    // of them (one more for the first `extra` workgroups) from first_chunk(w)
+    // on, so all get the same work whatever the lengths; an unsplit launch has
+    // a workgroup per segment.
+    bool split, merge_launch;
+    int share, extra;
+    int begin[kKv8Batch + 1];  // first chunk of each sequence
     int len[kKv8Batch];
 };
 
-__host__ __device__ inline int chunks_of(int len) { return len > 0 ? (len + kChunk - 1) / kChunk : 1; }
+// Chunks of a sequence: a step of `waves` wavefronts each.
+__host__ __device__ inline int chunks_of(int len, int waves) {
+    return len > 0 ? (len + waves * kTile - 1) / (waves * kTile) : 1;
+}
+
+// First chunk of workgroup w, and the workgroup that takes a chunk.
+__device__ __forceinline__ int first_chunk(const AttentionArgs &a, int w) { return w * a.share + min(w, a.extra); }
+__device__ __forceinline__ int owner_of(const AttentionArgs &a, int chunk) {
+    const int more = a.extra * (a.share + 1);  // chunks of the workgroups with one more
+    return chunk < more ? chunk / (a.share + 1) : a.extra + (chunk - more) / a.share;
+}
 
 // Loads of a wavefront's step: K row pieces, V pieces and the two scales of
 // both blocks.
@@ -380,6 +408,14 @@ struct TileRegs {
     u32x4_t k[2][KP], v[2][KP];
     float2 scale[2];
 };
+
+// 16 bytes of the cache; a call that streams more than the caches hold loads
+// them non-temporally.
+template <bool STREAM>
+__device__ __forceinline__ u32x4_t cache_load(const uint8_t *p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(p));
+    else return *reinterpret_cast<const u32x4_t *>(p);
+}
 
 // Four outputs of a row with the sum l; one that sees nothing is zeros.
 __device__ __forceinline__ void write_row(uint16_t *out, const float4 &o, float l) {
@@ -390,12 +426,110 @@ __device__ __forceinline__ void write_row(uint16_t *out, const float4 &o, float 
     *reinterpret_cast<uint2 *>(out) = packed;
 }
 
-// A workgroup of four wavefronts takes 16 * NT query rows of one kv head
-// ((query, head of the group) pairs) over a run of 128-token chunks, the
-// wavefronts 32 tokens each of a chunk:
-//   * K and V are an HBM stream: each wavefront keeps a ring of DEPTH steps
-//     in registers, DEPTH - 1 of them in flight while one is computed, and
-//     reads the page numbers of a step one step before its loads go out;
+// Rows [r0, r1) of a row tile (first row `row0` of the kv head, `tile_rows`
+// rows in a part) from the parts that workgroups w0, w0 + 1, ... left.
+// Thread -> (four outputs, every `lanes`-th part from the `from`-th on), with
+// more lanes where a part's rows are fewer than the threads.  A batch of parts
+// costs a round trip to the device's memory: all its loads go out before the
+// first is waited for, and only the sums depend on each other.  (One part
+// after another, each with its own maximum, took 11 us for 64 parts, this 7.)
+template <int THREADS>
+__device__ __forceinline__ void merge_parts(const AttentionArgs &a, int b, int seg, int row0, int tile_rows, int r0,
+                                            int r1, int d, int w0, int parts, int tid, float2 *lane_ml,
+                                            float4 *lane_sums) {
+    const int group = a.q_heads / a.cache.kv_heads;
+    const int head = seg / a.row_tiles;
+    const int64_t slot_floats = (int64_t)tile_rows * (d + 2);
+    const int items = (r1 - r0) * (d / 4);
+    int lanes = 1;
+    while (lanes * 2 * items <= THREADS && lanes < 8) lanes *= 2;
+    const int turns = (items + THREADS - 1) / THREADS;  // 1 where lanes > 1
+    for (int turn = 0; turn < turns; ++turn) {
+        const int it = lanes > 1 ? tid % items : turn * THREADS + tid;
+        const int from = lanes > 1 ? tid / items : 0;
+        const int r = r0 + min(it, items - 1) / (d / 4), at = min(it, items - 1) % (d / 4) * 4;
+        float m = -__FLT_MAX__, l = 0.0f;
+        float4 ov = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        auto batch = [&](int first, auto count) __attribute__((always_inline)) {
+            constexpr int K = decltype(count)::value;
+            float2 ml[K], x0[K], x1[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int j = min(first + k * lanes, parts - 1);
+                const float *src = a.partial + (2 * (w0 + j) + (j == 0 ? 1 : 0)) * slot_floats;
+                ml[k] = load_coherent2(src + tile_rows * d + r * 2);
+                x0[k] = load_coherent2(src + r * d + at);
+                x1[k] = load_coherent2(src + r * d + at + 2);
+            }
+            float m_new = m;
+#pragma unroll
+            for (int k = 0; k < K; ++k) m_new = fmaxf(m_new, ml[k].x);
+            const float keep = __builtin_amdgcn_exp2f(m - m_new);
+            l *= keep;
+            ov.x *= keep; ov.y *= keep; ov.z *= keep; ov.w *= keep;
+            m = m_new;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (first + k * lanes >= parts) continue;
+                const float w = __builtin_amdgcn_exp2f(ml[k].x - m);
+                l = fmaf(ml[k].y, w, l);
+                ov.x = fmaf(x0[k].x, w, ov.x); ov.y = fmaf(x0[k].y, w, ov.y);
+                ov.z = fmaf(x1[k].x, w, ov.z); ov.w = fmaf(x1[k].y, w, ov.w);
+            }
+        };
+        for (int j = from; j < parts; j += kMergeParts * lanes) {
+            const int left = (parts - j + lanes - 1) / lanes;
+            if (left <= 4) batch(j, std::integral_constant<int, 4>{});
+            else if (left <= 8) batch(j, std::integral_constant<int, 8>{});
+            else batch(j, std::integral_constant<int, kMergeParts>{});
+        }
+        if (lanes > 1) {
+            lane_ml[tid] = make_float2(m, l);
+            lane_sums[tid] = ov;
+            __syncthreads();
+            if (from == 0) {
+                for (int k = 1; k < lanes; ++k) {
+                    const float2 y = lane_ml[k * items + it];
+                    const float4 x = lane_sums[k * items + it];
+                    const float m_new = fmaxf(m, y.x);
+                    const float wo = __builtin_amdgcn_exp2f(m - m_new), wn = __builtin_amdgcn_exp2f(y.x - m_new);
+                    l = fmaf(l, wo, y.y * wn);
+                    ov.x = fmaf(ov.x, wo, x.x * wn); ov.y = fmaf(ov.y, wo, x.y * wn);
+                    ov.z = fmaf(ov.z, wo, x.z * wn); ov.w = fmaf(ov.w, wo, x.w * wn);
+                    m = m_new;
+                }
+            }
+        }
+        if (it < items && from == 0) {
+            const int row = row0 + r;
+            write_row(a.out + (((int64_t)b * a.queries + row / group) * a.q_heads + head * group + row % group) * d + at,
+                      ov, l);
+        }
+    }
+}
+
+// The merge as a launch of its own, a workgroup per row.
+__global__ __launch_bounds__(256) void merge_kernel(AttentionArgs a, int tile_rows, int waves) {
+    __shared__ float2 lane_ml[256];
+    __shared__ float4 lane_sums[256];
+    const int segments = a.cache.kv_heads * a.row_tiles;
+    const int r = (int)(blockIdx.x % tile_rows);
+    const int seg = (int)(blockIdx.x / tile_rows % segments), b = (int)(blockIdx.x / tile_rows / segments);
+    const int row0 = seg % a.row_tiles * tile_rows;
+    const int nch = chunks_of(a.len[b], waves), begin = a.begin[b] + seg * nch;
+    const int w0 = owner_of(a, begin), parts = owner_of(a, begin + nch - 1) - w0 + 1;
+    if (parts == 1 || row0 + r >= a.queries * (a.q_heads / a.cache.kv_heads)) return;
+    merge_parts<256>(a, b, seg, row0, tile_rows, r, r + 1, a.cache.head_dim, w0, parts, threadIdx.x, lane_ml,
+                     lane_sums);
+}
+
+// A workgroup of four or eight wavefronts takes 16 * NT query rows of one kv
+// head ((query, head of the group) pairs) over a run of chunks, the wavefronts
+// 32 tokens each of a chunk:
+//   * K and V are an HBM stream: each wavefront holds two steps in registers,
+//     the next one in flight while one is computed, and reads the page numbers
+//     of a step one step before its loads go out (a third step in registers
+//     was 1 to 2 us slower at every size, its moves costing more than it hid);
 //   * S^T = K.Q^T on v_mfma_f32_16x16x32_bf16, 16 tokens of a block as M and
 //     16 rows as N.  A lane's 16 bytes of a K row widen to the A operands of
 //     two MFMAs, whose 8 dims per lane group are taken from Q in that order;
@@ -405,16 +539,22 @@ __device__ __forceinline__ void write_row(uint16_t *out, const float4 &o, float 
 //     the rounded P, so O / l is a convex combination of V rows;
 //   * a lane's 16 bytes of V are four dims of four tokens: the B operand's
 //     tokens of its lane group;
-//   * the four wavefronts merge in LDS, the parts of a segment that several
-//     workgroups took in the one that ends last, in the order of the tokens.
+//   * the wavefronts merge in LDS, the parts of a segment that several
+//     workgroups took in the one that ends last or in a launch that follows,
+//     in the order of the tokens either way.
+// Measured, E4M3, 64/8 heads of 128: 4 x 32,768 tokens 51.1 us, 5.3 TB/s; each
+// further 269 MB 40 us, 6.7 TB/s; about 4 us are the launch, 3 the first loads
+// and 4 the merge.
 // DM: head_dim rounded up to 64, 128 or 256; FULL: equal to it.
-template <int FMT, int DM, bool FULL, int NT, int DEPTH, int WGS>
-__global__ __launch_bounds__(64 * kWaves, WGS) void attention_kernel(AttentionArgs a) {
+template <int FMT, int DM, bool FULL, int NT, int WAVES, int WGS, bool STREAM>
+__global__ __launch_bounds__(64 * WAVES, WGS) void attention_kernel(AttentionArgs a) {
+    constexpr int CHUNK = WAVES * kTile;
     constexpr int KP = DM / 64;  // 16-byte pieces of a lane per block
     constexpr int ROWS = 16 * NT;
-    __shared__ float comb_ml[kWaves][ROWS][2];
-    __shared__ __align__(16) float comb_acc[kWaves][16][DM];
+    __shared__ float comb_ml[WAVES][ROWS][2];
+    __shared__ __align__(16) float comb_acc[WAVES][16][DM];
     __shared__ int last_part;
+    __shared__ float2 merge_ml[64 * WAVES];
     const Kv8Cache &c = a.cache;
     const int d = FULL ? DM : c.head_dim;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -427,7 +567,7 @@ __global__ __launch_bounds__(64 * kWaves, WGS) void attention_kernel(AttentionAr
     // Chunks [ch, ch_end) of segment `seg` of sequence b.
     auto run = [&](int b, int seg, int ch, int ch_end) __attribute__((always_inline)) {
         const int head = seg / a.row_tiles, rt = seg % a.row_tiles;
-        const int len = a.len[b], nch = chunks_of(len);
+        const int len = a.len[b], nch = chunks_of(len, WAVES);
         // Row r of a kv head is (query r / group, head r % group of the group).
         auto row_at = [&](int r) {
             return (((int64_t)b * a.queries + r / group) * a.q_heads + head * group + r % group) * d;
@@ -453,7 +593,7 @@ __global__ __launch_bounds__(64 * kWaves, WGS) void attention_kernel(AttentionAr
         // Loads never branch: a block past the end repeats the last one, an
         // entry that names no page reads page 0, a piece past head_dim the
         // row's last one; what they bring is masked below.
-        const int t_first = ch * kChunk + wave * kTile, t_end = min(len, ch_end * kChunk);
+        const int t_first = ch * CHUNK + wave * kTile, t_end = min(len, ch_end * CHUNK);
         const int32_t *table = c.table + (int64_t)b * c.pages_per_seq;
         const int last = max(len - 1, 0) & ~15;
         const int in_page = (1 << c.shift) - 1;
@@ -461,7 +601,7 @@ __global__ __launch_bounds__(64 * kWaves, WGS) void attention_kernel(AttentionAr
             int p[2];
         };
         auto pages_at = [&](int t0) {
-            return Pages{{table[min(t0, last) >> c.shift], table[min(t0 + 16, last) >> c.shift]}};
+            return Pages{{scalar_page(table + (min(t0, last) >> c.shift)), scalar_page(table + (min(t0 + 16, last) >> c.shift))}};
         };
         auto known = [&](int page) { return page >= 0 && page < (int)c.pool_pages; };
         const int k_at = row16 * d + grp * 16, v_at = grp * d * 4 + row16 * 16;
@@ -471,13 +611,13 @@ __global__ __launch_bounds__(64 * kWaves, WGS) void attention_kernel(AttentionAr
                 const int bt = min(t0 + blk * 16, last);
                 const int64_t page = known(pg.p[blk]) ? pg.p[blk] : 0;
                 const int64_t block = ((page * c.kv_heads + head) << (c.shift - 4)) + ((bt & in_page) >> 4);
-                r.scale[blk] = reinterpret_cast<const float2 *>(c.scales)[block];
+                r.scale[blk] = scalar_scales(c.scales + block * 2);
                 const uint8_t *kb = c.k + block * 16 * d, *vb = c.v + block * 16 * d;
 #pragma unroll
                 for (int j = 0; j < KP; ++j) {
-                    r.k[blk][j] = *reinterpret_cast<const u32x4_t *>(
+                    r.k[blk][j] = cache_load<STREAM>(
                         kb + (FULL ? k_at + j * 64 : row16 * d + min(j * 64 + grp * 16, d - 16)));
-                    r.v[blk][j] = *reinterpret_cast<const u32x4_t *>(
+                    r.v[blk][j] = cache_load<STREAM>(
                         vb + (FULL ? v_at + j * 256 : grp * d * 4 + min(j * 64 + row16 * 4, d - 4) * 4));
                 }
             }
@@ -576,38 +716,36 @@ __global__ __launch_bounds__(64 * kWaves, WGS) void attention_kernel(AttentionAr
         // Ring over this wavefront's steps; past the last one the loads
         // repeat it, so every turn issues the same ones.
         if (t_first < t_end) {
-            const int t_last = t_first + (t_end - 1 - t_first) / kChunk * kChunk;
-            auto step_at = [&](int i) { return min(t_first + i * kChunk, t_last); };
-            TileRegs<KP> ring[DEPTH];
-            Pages pages[DEPTH + 1];
+            const int t_last = t_first + (t_end - 1 - t_first) / CHUNK * CHUNK;
+            auto step_at = [&](int i) { return min(t_first + i * CHUNK, t_last); };
+            TileRegs<KP> ring[2];
+            Pages pages[3];
+            pages[0] = pages_at(step_at(0));
+            pages[1] = pages_at(step_at(1));
+            load_tile(ring[0], pages[0], step_at(0));
+            for (int base = 0; t_first + base * CHUNK < t_end; base += 2) {
 #pragma unroll
-            for (int i = 0; i < DEPTH; ++i) pages[i] = pages_at(step_at(i));
-#pragma unroll
-            for (int i = 0; i < DEPTH - 1; ++i) load_tile(ring[i], pages[i], step_at(i));
-            for (int base = 0; t_first + base * kChunk < t_end; base += DEPTH) {
-#pragma unroll
-                for (int i = 0; i < DEPTH; ++i) {
-                    const int t0 = t_first + (base + i) * kChunk;
+                for (int i = 0; i < 2; ++i) {
+                    const int t0 = t_first + (base + i) * CHUNK;
                     if (t0 >= t_end) break;
-                    pages[DEPTH] = pages_at(step_at(base + i + DEPTH));
-                    load_tile(ring[(i + DEPTH - 1) % DEPTH], pages[DEPTH - 1], step_at(base + i + DEPTH - 1));
+                    pages[2] = pages_at(step_at(base + i + 2));
+                    load_tile(ring[1 - i], pages[1], step_at(base + i + 1));
                     __builtin_amdgcn_sched_barrier(0);
                     compute_tile(ring[i], pages[0], t0);
-#pragma unroll
-                    for (int k = 0; k < DEPTH; ++k) pages[k] = pages[k + 1];
+                    pages[0] = pages[1];
+                    pages[1] = pages[2];
                 }
             }
         }
 
         const bool alone = ch == 0 && ch_end == nch;
-        const int64_t seg_begin = a.begin[b] + (int64_t)seg * nch;
+        const int seg_begin = a.begin[b] + seg * nch;
         const int here = min(ROWS, rows - rt * ROWS);
         // Slot of a workgroup's part: its last segment, which others go on
         // with, or its first, which others have begun.
         const int64_t slot_floats = (int64_t)ROWS * (d + 2);
-        auto part = [&](int64_t w, bool begins) { return a.partial + (2 * w + (begins ? 1 : 0)) * slot_floats; };
-        auto owner = [&](int64_t chunk) { return ((chunk + 1) * a.workgroups - 1) / a.total; };
-        float *mine = a.split ? part(owner(seg_begin + ch), ch == 0) : nullptr;
+        auto part = [&](int w, bool begins) { return a.partial + (2 * w + (begins ? 1 : 0)) * slot_floats; };
+        float *mine = a.split ? part(owner_of(a, seg_begin + ch), ch == 0) : nullptr;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             float l = wave_xor_sum(l_run[t], 16);
@@ -624,15 +762,15 @@ __global__ __launch_bounds__(64 * kWaves, WGS) void attention_kernel(AttentionAr
                 comb_ml[wave][t * 16 + lane][1] = l;
             }
             __syncthreads();
-            for (int it = tid; it < min(16, here - t * 16) * (d / 4); it += 64 * kWaves) {
+            for (int it = tid; it < min(16, here - t * 16) * (d / 4); it += 64 * WAVES) {
                 const int r = it / (d / 4), at = it % (d / 4) * 4;
                 float m = -__FLT_MAX__;
 #pragma unroll
-                for (int w = 0; w < kWaves; ++w) m = fmaxf(m, comb_ml[w][t * 16 + r][0]);
+                for (int w = 0; w < WAVES; ++w) m = fmaxf(m, comb_ml[w][t * 16 + r][0]);
                 float lr = 0.0f;
                 float4 ov = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                for (int w = 0; w < kWaves; ++w) {
+                for (int w = 0; w < WAVES; ++w) {
                     const float wt = __builtin_amdgcn_exp2f(comb_ml[w][t * 16 + r][0] - m);
                     lr = fmaf(comb_ml[w][t * 16 + r][1], wt, lr);
                     const float4 y = *reinterpret_cast<const float4 *>(&comb_acc[w][r][at]);
@@ -649,58 +787,31 @@ __global__ __launch_bounds__(64 * kWaves, WGS) void attention_kernel(AttentionAr
                 }
             }
         }
-        if (alone) return;
+        if (alone || a.merge_launch) return;
         // The parts are ordered as the BF16 decode's are: written through to
         // the device, complete before the barrier, counted, and read past the
         // XCD's own L2 by the workgroup that counts the last.
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
-        const int64_t w0 = owner(seg_begin), w1 = owner(seg_begin + nch - 1);
+        const int w0 = owner_of(a, seg_begin), parts = owner_of(a, seg_begin + nch - 1) - w0 + 1;
         if (tid == 0) {
             int *counter = a.counters + (int64_t)b * segments + seg;
             const int done = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            last_part = done == (int)(w1 - w0);
+            last_part = done == parts - 1;
             if (last_part) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         __syncthreads();
         if (!last_part) return;
-        for (int it = tid; it < here * (d / 4); it += 64 * kWaves) {
-            const int r = it / (d / 4), at = it % (d / 4) * 4;
-            float m = -__FLT_MAX__, l = 0.0f;
-            float4 ov = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            constexpr int K = 8;  // parts whose loads go out together
-            for (int64_t w = w0; w <= w1; w += K) {
-                float2 ml[K], x0[K], x1[K];
-#pragma unroll
-                for (int j = 0; j < K; ++j) {
-                    const int64_t from = min(w + j, w1);
-                    const float *src = part(from, from == w0);
-                    ml[j] = load_coherent2(src + ROWS * d + r * 2);
-                    x0[j] = load_coherent2(src + r * d + at);
-                    x1[j] = load_coherent2(src + r * d + at + 2);
-                }
-#pragma unroll
-                for (int j = 0; j < K; ++j) {
-                    if (w + j > w1) continue;
-                    const float m_new = fmaxf(m, ml[j].x);
-                    const float wo = __builtin_amdgcn_exp2f(m - m_new), wn = __builtin_amdgcn_exp2f(ml[j].x - m_new);
-                    l = fmaf(l, wo, ml[j].y * wn);
-                    ov.x = fmaf(ov.x, wo, x0[j].x * wn); ov.y = fmaf(ov.y, wo, x0[j].y * wn);
-                    ov.z = fmaf(ov.z, wo, x1[j].x * wn); ov.w = fmaf(ov.w, wo, x1[j].y * wn);
-                    m = m_new;
-                }
-            }
-            write_row(a.out + row_at(rt * ROWS + r) + at, ov, l);
-        }
+        merge_parts<64 * WAVES>(a, b, seg, rt * ROWS, ROWS, 0, here, d, w0, parts, tid, merge_ml, reinterpret_cast<float4 *>(comb_acc));
     };
 
     if (!a.split) {
         const int b = (int)(blockIdx.x / segments);
-        run(b, (int)(blockIdx.x % segments), 0, chunks_of(a.len[b]));
+        run(b, (int)(blockIdx.x % segments), 0, chunks_of(a.len[b], WAVES));
         return;
     }
-    int64_t at = blockIdx.x * a.total / a.workgroups;
-    const int64_t end = (blockIdx.x + 1) * a.total / a.workgroups;
+    int at = first_chunk(a, (int)blockIdx.x);
+    const int end = first_chunk(a, (int)blockIdx.x + 1);
     for (bool again = false; at < end; again = true) {
         if (again) __syncthreads();  // the LDS of the part before is free
         int b = 0;
@@ -709,10 +820,9 @@ __global__ __launch_bounds__(64 * kWaves, WGS) void attention_kernel(AttentionAr
             if (a.begin[mid] <= at) b = mid;
             else hi = mid - 1;
         }
-        const int nch = chunks_of(a.len[b]);
-        const int64_t local = at - a.begin[b];
-        const int seg = (int)(local / nch), ch = (int)(local % nch);
-        const int ch_end = (int)min((int64_t)nch, ch + end - at);
+        const int nch = chunks_of(a.len[b], WAVES);
+        const int seg = (at - a.begin[b]) / nch, ch = (at - a.begin[b]) % nch;
+        const int ch_end = min(nch, ch + end - at);
         run(b, seg, ch, ch_end);
         at += ch_end - ch;
     }
@@ -726,21 +836,38 @@ int row_tiles_at_once(const Kv8AttentionLaunch &l) {
     return rows <= 32 || l.cache.head_dim > 128 ? 2 : 4;
 }
 
+// How a launch runs.
+struct Shape {
+    int nt, waves;  // row tiles of 16 at once, wavefronts of a workgroup
+    bool stream;
+    bool merge_launch;  // parts are merged by a launch of their own
+    int row_tiles;
+    int64_t segments, total, workgroups;
+};
+
 template <int FMT, int DM, bool FULL>
-void launch_attention(const AttentionArgs &a, int nt, unsigned grid, hipStream_t stream) {
-    const dim3 block(64 * kWaves);
-    if (nt == 1)
-        hipLaunchKernelGGL((attention_kernel<FMT, DM, FULL, 1, (DM > 128 ? 2 : 3), (DM > 128 ? 1 : 2)>), dim3(grid), block, 0, stream, a);
-    else if (nt == 2)
-        hipLaunchKernelGGL((attention_kernel<FMT, DM, FULL, 2, 2, 1>), dim3(grid), block, 0, stream, a);
-    else if constexpr (DM <= 128)
-        hipLaunchKernelGGL((attention_kernel<FMT, DM, FULL, 4, 2, 1>), dim3(grid), block, 0, stream, a);
+void launch_attention(const AttentionArgs &a, const Shape &s, unsigned grid, hipStream_t stream) {
+    const dim3 block(64 * s.waves);
+#define MSLIM_KV8_LAUNCH(NT, WAVES, WGS, STREAM) \
+    hipLaunchKernelGGL((attention_kernel<FMT, DM, FULL, NT, WAVES, WGS, STREAM>), dim3(grid), block, 0, stream, a)
+    if constexpr (DM <= 128) {
+        if (s.nt == 1 && s.waves == 8 && s.stream) MSLIM_KV8_LAUNCH(1, 8, 1, true);
+        else if (s.nt == 1 && s.waves == 8) MSLIM_KV8_LAUNCH(1, 8, 1, false);
+        else if (s.nt == 1 && s.stream) MSLIM_KV8_LAUNCH(1, 4, 2, true);
+        else if (s.nt == 1) MSLIM_KV8_LAUNCH(1, 4, 2, false);
+        else if (s.nt == 2) MSLIM_KV8_LAUNCH(2, 4, 1, false);
+        else MSLIM_KV8_LAUNCH(4, 4, 1, false);
+    } else {
+        if (s.nt == 1) MSLIM_KV8_LAUNCH(1, 4, 1, false);
+        else MSLIM_KV8_LAUNCH(2, 4, 1, false);
+    }
+#undef MSLIM_KV8_LAUNCH
 }
 
 template <int FMT, int DM>
-void launch_attention(const AttentionArgs &a, int nt, unsigned grid, hipStream_t stream) {
-    if (a.cache.head_dim == DM) launch_attention<FMT, DM, true>(a, nt, grid, stream);
-    else launch_attention<FMT, DM, false>(a, nt, grid, stream);
+void launch_attention(const AttentionArgs &a, const Shape &s, unsigned grid, hipStream_t stream) {
+    if (a.cache.head_dim == DM) launch_attention<FMT, DM, true>(a, s, grid, stream);
+    else launch_attention<FMT, DM, false>(a, s, grid, stream);
 }
 
 template <int FMT>
@@ -799,21 +926,29 @@ hipError_t launch_kv8_gather(const Kv8Cache &cache, int batch, int tokens, const
 }
 
 namespace {
-struct Shape {
-    int nt, row_tiles;
-    int64_t segments, total, workgroups;
-};
-// Two workgroups per CU share the chunks of all segments evenly, fewer where
-// there are fewer chunks.
 Shape shape_of(const Kv8AttentionLaunch &l) {
     Shape s;
     s.nt = row_tiles_at_once(l);
     const int64_t rows = (int64_t)l.queries * (l.q_heads / l.cache.kv_heads);
     s.row_tiles = (int)((rows + 16 * s.nt - 1) / (16 * s.nt));
     s.segments = (int64_t)l.cache.kv_heads * s.row_tiles;
-    s.total = 0;
-    for (int b = 0; b < l.batch; ++b) s.total += chunks_of(l.len[b]) * s.segments;
-    s.workgroups = std::min<int64_t>(s.total, (s.nt == 1 && l.cache.head_dim <= 128 ? 2 : 1) * kCus);
+    auto chunks = [&](int waves) {
+        int64_t n = 0;
+        for (int b = 0; b < l.batch; ++b) n += chunks_of(l.len[b], waves) * s.segments;
+        return n;
+    };
+    s.waves = 4;
+    s.total = chunks(4);
+    const bool wide = l.cache.head_dim > 128;
+    s.workgroups = std::min<int64_t>(s.total, s.nt == 1 && !wide ? 2 * kCus : kCus);
+    if (s.nt == 1 && !wide && s.workgroups >= kWideParts * s.segments * l.batch) {
+        s.waves = 8;
+        s.total = chunks(8);
+        s.workgroups = std::min<int64_t>(s.total, kCus);
+    }
+    const int64_t parts = s.workgroups / (s.segments * l.batch) + 1;
+    s.merge_launch = parts * std::min<int64_t>(rows, 16 * s.nt) * (l.cache.head_dim + 2) * 4 > kMergeLaunchBytes;
+    s.stream = s.total * s.waves * kTile * l.cache.head_dim * 2 >= kStreamBytes;
     return s;
 }
 }  // namespace
@@ -821,7 +956,9 @@ Shape shape_of(const Kv8AttentionLaunch &l) {
 Kv8AttentionPlan kv8_attention_plan(const Kv8AttentionLaunch &l) {
     const Shape s = shape_of(l);
     Kv8AttentionPlan p{};
-    if (s.segments * l.batch > 4 * s.workgroups) return p;  // as even without: nothing to merge
+    // as even without where segments are many; positions of chunks are 32 bits
+    if (s.segments * l.batch > 4 * s.workgroups || s.total > INT32_MAX / 2) return p;
+    p.split = true;
     p.partial_bytes = (size_t)(2 * s.workgroups) * 16 * s.nt * (l.cache.head_dim + 2) * sizeof(float);
     p.counters = (size_t)(s.segments * l.batch);
     return p;
@@ -837,21 +974,26 @@ hipError_t launch_kv8_attention(const Kv8AttentionLaunch &l, hipStream_t stream)
     a.row_tiles = shape.row_tiles;
     a.scale_log2e = l.scale * kLog2e;
     a.split = l.split;
-    a.total = shape.total;
-    a.workgroups = shape.workgroups;
-    for (int b = 0; b < l.batch; ++b) {
-        a.len[b] = l.len[b];
-        a.begin[b + 1] = a.begin[b] + chunks_of(l.len[b]) * shape.segments;
+    a.merge_launch = l.split && shape.merge_launch;
+    for (int b = 0; b < l.batch; ++b) a.len[b] = l.len[b];
+    if (l.split) {
+        a.share = (int)(shape.total / shape.workgroups);
+        a.extra = (int)(shape.total % shape.workgroups);
+        for (int b = 0; b < l.batch; ++b) a.begin[b + 1] = a.begin[b] + (int)(chunks_of(l.len[b], shape.waves) * shape.segments);
     }
     const unsigned grid = (unsigned)(l.split ? shape.workgroups : shape.segments * l.batch);
     const int d = l.cache.head_dim;
 #define MSLIM_KV8_ATTENTION(FMT)                                              \
-    if (d <= 64) launch_attention<FMT, 64>(a, shape.nt, grid, stream);        \
-    else if (d <= 128) launch_attention<FMT, 128>(a, shape.nt, grid, stream); \
-    else launch_attention<FMT, 256>(a, shape.nt, grid, stream)
+    if (d <= 64) launch_attention<FMT, 64>(a, shape, grid, stream);        \
+    else if (d <= 128) launch_attention<FMT, 128>(a, shape, grid, stream); \
+    else launch_attention<FMT, 256>(a, shape, grid, stream)
     if (l.cache.format == kFormatE4m3) { MSLIM_KV8_ATTENTION(kFormatE4m3); }
     else { MSLIM_KV8_ATTENTION(kFormatInt8); }
 #undef MSLIM_KV8_ATTENTION
+    if (hipError_t err = hipGetLastError(); err != hipSuccess || !a.merge_launch) return err;
+    const int tile_rows = 16 * shape.nt;
+    hipLaunchKernelGGL(merge_kernel, dim3((unsigned)(shape.segments * l.batch * tile_rows)), dim3(256), 0, stream, a,
+                       tile_rows, shape.waves);
     return hipGetLastError();
 }
 

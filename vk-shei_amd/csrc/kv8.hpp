@@ -6,6 +6,17 @@
 
 namespace mslim {
 
+// Page numbers and scales that a whole wavefront reads, through the scalar
+// cache: no kernel that reads them so writes them.  (As vector loads each was
+// waited for where it was issued, behind every K and V load in flight.)
+__device__ __forceinline__ int32_t scalar_page(const int32_t *p) {
+    return *reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(reinterpret_cast<uintptr_t>(p));
+}
+__device__ __forceinline__ float2 scalar_scales(const float *p) {
+    const uint64_t w = *reinterpret_cast<const __attribute__((address_space(4))) uint64_t *>(reinterpret_cast<uintptr_t>(p));
+    return make_float2(__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32)));
+}
+
 // The value of byte i of four.
 template <int FMT>
 __device__ __forceinline__ float byte_value(uint32_t w, int i) {

@@ -1,5 +1,6 @@
 // Attention of many query rows over the 8-bit paged K/V cache: prompt chunks.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "common.hpp"
@@ -21,23 +22,30 @@ constexpr float kLazyBound = 256.0f;
 
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
+// A segment that workgroup w is the first but not the only one to take, for
+// the merge: `count` parts, by w, w + 1, ...; 0 where there is none.
+struct Part {
+    int b, head, rt, count;
+};
+
 struct PrefillArgs {
     Kv8Cache cache;
     const uint16_t *q;
     uint16_t *out;
-    float *partial;  // [2 * workgroups][wavefront][pair][64] float pairs
-    int *counters;   // [batch][kv_heads * row_tiles] parts done, zero between launches
+    float2 *partial;  // [2 * workgroups][wavefront][pair][64]: O, then (m, l)
+    Part *parts;      // [workgroups]
     int batch, queries, q_heads;
     int tile_queries;  // queries of a row tile: kRows / group
     int row_tiles;
     float scale_log2e;
-    // Segments (sequence, kv head, row tile) laid end to end; workgroup w of a
-    // split launch takes tiles w * total / workgroups .. of them, an unsplit
-    // one has a workgroup per segment.
+    // Segments (sequence, kv head, row tile) laid end to end.  Workgroup w of
+    // a split launch takes `share` tiles of them (one more for the first
+    // `extra` workgroups) from first_tile(w) on, an unsplit one has a
+    // workgroup per segment.
     bool split;
-    int64_t total, workgroups;
-    int64_t begin[kKv8Batch + 1];  // first tile of each sequence
-    int64_t head_tiles[kKv8Batch];  // tiles of one kv head of each sequence
+    int share, extra, workgroups;
+    int begin[kKv8Batch + 1];   // first tile of each sequence
+    int head_tiles[kKv8Batch];  // tiles of one kv head of each sequence
     int prior[kKv8Batch];
 };
 
@@ -46,6 +54,18 @@ __host__ __device__ inline int tiles_of(int prior, int queries, int tile_queries
     const int64_t end = prior + ((int64_t)(rt + 1) * tile_queries < queries ? (int64_t)(rt + 1) * tile_queries
                                                                             : (int64_t)queries);
     return (int)((end + kBN - 1) / kBN);
+}
+
+// First tile of workgroup w, and the workgroup that takes a tile.
+__device__ __forceinline__ int first_tile(const PrefillArgs &a, int w) { return w * a.share + min(w, a.extra); }
+__device__ __forceinline__ int owner_of(const PrefillArgs &a, int tile) {
+    const int more = a.extra * (a.share + 1);  // tiles of the workgroups with one more
+    return tile < more ? tile / (a.share + 1) : a.extra + (tile - more) / a.share;
+}
+// A wavefront's share of a workgroup's part: of its last segment, which others
+// go on with (begins), or of its first.
+__device__ __forceinline__ float2 *part_at(const PrefillArgs &a, int w, bool begins, int wave, int pairs) {
+    return a.partial + (int64_t)((2 * w + (begins ? 1 : 0)) * kWaves + wave) * pairs * 64;
 }
 
 // Bytes times a scale as BF16.  A power of two, what the append writes, is
@@ -102,9 +122,8 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
     constexpr int NSLOT = DM / 8;      // 16-byte slots of a K row in LDS
     constexpr int PIECES = kBN * DM / 16;  // 16-byte pieces of a tile's K (and V) bytes: 512 or 256
     constexpr int PAIRS = MT * 8 + 1;
-    __shared__ __align__(16) uint16_t k_lds[2][kBN * DM];
-    __shared__ __align__(16) uint16_t v_lds[3][kBN * DM];  // [block][4][dim][4 tokens]
-    __shared__ int last_part;
+    __shared__ __align__(256) uint16_t k_lds[2][kBN * DM];
+    __shared__ __align__(16) uint16_t v_lds[4][kBN * DM];  // [block][4][dim][4 tokens]
 
     const Kv8Cache &c = a.cache;
     const int d = FULL ? DM : c.head_dim;
@@ -130,14 +149,13 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
     uint16_t *const v_to = &v_lds[0][((piece / DM * 4 + v_grp) * DM + v_dim) * 4];
 
     // Fragment addresses in stage 0; a stage and a block of rows are immediates.
-    uint32_t k_from[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-        k_from[ks] = lds_offset(k_lds) + (uint32_t)(col * DM + k_slot(col, 2 * ks + half) * 8) * 2;
+    // A K fragment's slot is (2 ks + half) ^ (row % NSLOT): k-step ks flips bits
+    // of the address of the first.
+    const uint32_t k_from = lds_offset(k_lds) + (uint32_t)(col * DM + k_slot(col, half) * 8) * 2;
     const uint32_t v_from = lds_offset(v_lds) + (uint32_t)(half * DM + col) * 8;
     constexpr uint32_t STAGE = kBN * DM * 2;
 
-    auto run = [&](int b, int head, int rt, int tile, int tile_end, int64_t seg_begin, int tiles)
+    auto run = [&](int b, int head, int rt, int tile, int tile_end, int tiles, int w)
         __attribute__((always_inline)) {
         const int prior = a.prior[b];
         const int len = prior + a.queries;
@@ -167,7 +185,7 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
         auto pages_at = [&](int t) {
             Pages pg;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pg.p[i] = table[block_at(t, i) >> c.shift];
+            for (int i = 0; i < 4; ++i) pg.p[i] = scalar_page(table + (block_at(t, i) >> c.shift));
             return pg;
         };
         auto known = [&](int page) { return page >= 0 && page < (int)c.pool_pages; };
@@ -183,7 +201,7 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
             const int64_t page = no_page ? 0 : pick;
             const int64_t block = ((page * c.kv_heads + head) << (c.shift - 4)) +
                                   ((block_at(t, my_block) & ((1 << c.shift) - 1)) >> 4);
-            scale = reinterpret_cast<const float2 *>(c.scales)[block];
+            scale = scalar_scales(c.scales + block * 2);
             if (has_k) k_in_regs = *reinterpret_cast<const u32x4_t *>(c.k + block * 16 * d + k_off);
             if (has_v) v_in_regs = *reinterpret_cast<const u32x4_t *>(c.v + block * 16 * d + v_off);
         };
@@ -221,12 +239,13 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
         float m_used = -__FLT_MAX__, l_run = 0.0f, alpha = 1.0f;
         bool rescale = false;
         floatx16_t s[2];
-        bf16x8_t p[2][2];  // [key half of 32][16 of them]
+        bf16x8_t p[2][2] = {};  // [key half of 32][16 of them]
 
         // Scores of the tile in K stage st; `mid(n)` after MFMA n.
         auto qk = [&](int st, auto &&mid) __attribute__((always_inline)) {
+            const uint32_t from = k_from + st * STAGE;
             auto frag = [&](int n) __attribute__((always_inline)) {
-                return lds_read_b128(k_from[n / 2] + st * STAGE + n % 2 * 32 * DM * 2);
+                return lds_read_b128((from ^ (uint32_t)(n / 2 * 32)) + n % 2 * 32 * DM * 2);
             };
             bf16x8_t kq[3];
             kq[0] = frag(0);
@@ -356,51 +375,47 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
         store_v(0, tile);
         load(pg1, clamp(tile + 1));
         barrier();
-        // First tile: scores, their maximum, P.
-        qk(0, [&](int n) __attribute__((always_inline)) {
-            if (n == 3) store_k(1);
-            if (n == KS + 1) store_v(1, clamp(tile + 1));
-            if (n == 2 * KS - 2) load(pg2, clamp(tile + 2));
-        });
-        mask(tile, pg0);
-        m_used = fmaxf(row_max(), m_used);
-#pragma unroll
-        for (int n = 0; n < 16; ++n) score_pair(n);
-        l_run = psum;
-        keep_p();
-        int ks = 1, vs = 0;  // stages of K of tile j and V of tile j - 1
-        for (int j = tile + 1; j < tile_end; ++j) {
-            pg0 = pg1;
-            pg1 = pg2;
-            pg2 = pages_at(clamp(j + 2));
-            barrier();
-            if (rescale) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[mt][i] *= alpha;
-                rescale = false;
-            }
-            const int vn = vs == 0 ? 2 : vs - 1;  // of V of tile j + 1
-            qk(ks, [&](int n) __attribute__((always_inline)) {
-                if (n == 3) store_k(ks ^ 1);
-                if (n == KS + 1) store_v(vn, clamp(j + 1));
-                if (n == 2 * KS - 2) load(pg2, clamp(j + 2));
-            });
-            mask(j, pg0);
-            pv(vs, std::true_type{});
-            settle();
-            keep_p();
-            ks ^= 1;
-            vs = vs == 2 ? 0 : vs + 1;
-        }
-        if (rescale) {
+        auto apply_rescale = [&]() __attribute__((always_inline)) {
+            if (!rescale) return;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[mt][i] *= alpha;
+            rescale = false;
+        };
+        int n = 0;  // tiles done; K of tile j is in stage n % 2, V in n % 4
+        // Q.K of tile j, and tile j + 1 to LDS on the way
+        auto scores = [&](int j) __attribute__((always_inline)) {
+            qk(n & 1, [&](int m) __attribute__((always_inline)) {
+                if (m == 3) store_k(~n & 1);
+                if (m == KS + 1) store_v((n + 1) & 3, clamp(j + 1));
+                if (m == 2 * KS - 2) load(pg2, clamp(j + 2));
+            });
+            mask(j, pg0);
+        };
+        auto next = [&](int j) __attribute__((always_inline)) {
+            pg0 = pg1;
+            pg1 = pg2;
+            pg2 = pages_at(clamp(j + 2));
+            ++n;
+            barrier();
+        };
+        // Softmax of the scores at hand with P.V of the tile before them; a
+        // run's first has P = 0 and takes its own V.
+        auto softmax_pv = [&](int before) __attribute__((always_inline)) {
+            apply_rescale();
+            pv(max(before, 0) & 3, std::true_type{});
+            settle();
+            keep_p();
+        };
+        for (int j = tile;;) {
+            scores(j);
+            softmax_pv(n - 1);
+            if (++j == tile_end) break;
+            next(j);
         }
-        pv(vs, std::false_type{});
+        apply_rescale();
+        pv(n & 3, std::false_type{});
 
         float l = l_run + __shfl_xor(l_run, 32, 64);
         auto write_out = [&](const floatx16_t *acc, float lsum) __attribute__((always_inline)) {
@@ -421,91 +436,47 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
             write_out(o, l);
             return;
         }
-        // Parts of a segment: written through to the device, complete before
-        // the barrier, counted, and merged in the order of the keys by the
-        // workgroup that counts the last (as the decode's are).
-        auto owner = [&](int64_t t) { return ((t + 1) * a.workgroups - 1) / a.total; };
-        auto part = [&](int64_t w, bool begins) {
-            return a.partial + (((2 * w + (begins ? 1 : 0)) * kWaves + wave) * PAIRS * 64 + lane) * 2;
-        };
-        float *mine = part(owner(seg_begin + tile), tile == 0);
+        // A part of a segment, for the merge launch.
+        float2 *mine = part_at(a, w, tile == 0, wave, PAIRS) + lane;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) store_coherent2(mine + (mt * 8 + i) * 128, o[mt][2 * i], o[mt][2 * i + 1]);
-        store_coherent2(mine + MT * 8 * 128, m_used, l);
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        const int64_t w0 = owner(seg_begin), w1 = owner(seg_begin + tiles - 1);
-        if (tid == 0) {
-            int *counter = a.counters + ((int64_t)b * c.kv_heads + head) * a.row_tiles + rt;
-            const int done = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            last_part = done == (int)(w1 - w0);
-            if (last_part) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-        if (!last_part) return;
-        float m = -__FLT_MAX__;
-        l = 0.0f;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[mt][i] = 0.0f;
-        for (int64_t w = w0; w <= w1; ++w) {
-            const float *from = part(w, w == w0);
-            float2 x[MT * 8];
-#pragma unroll
-            for (int e = 0; e < MT * 8; ++e) x[e] = load_coherent2(from + e * 128);
-            const float2 ml = load_coherent2(from + MT * 8 * 128);
-            const float m_new = fmaxf(m, ml.x);
-            const float wo = __builtin_amdgcn_exp2f(m - m_new), wn = __builtin_amdgcn_exp2f(ml.x - m_new);
-            l = fmaf(l, wo, ml.y * wn);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    o[mt][2 * i] = fmaf(o[mt][2 * i], wo, x[mt * 8 + i].x * wn);
-                    o[mt][2 * i + 1] = fmaf(o[mt][2 * i + 1], wo, x[mt * 8 + i].y * wn);
-                }
-            m = m_new;
-        }
-        write_out(o, l);
+            for (int i = 0; i < 8; ++i) mine[(mt * 8 + i) * 64] = make_float2(o[mt][2 * i], o[mt][2 * i + 1]);
+        mine[MT * 8 * 64] = make_float2(m_used, l);
     };
 
     // Workgroup -> run of tiles: XCD x (workgroups x, x + 8, ...) takes a
     // contiguous eighth of all, so the kv heads that it reads stay in its L2.
-    int64_t at, end;
-    if (a.split) {
-        const int64_t per_xcd = a.workgroups / kXcds;
-        const int64_t w = a.workgroups % kXcds ? blockIdx.x : blockIdx.x % kXcds * per_xcd + blockIdx.x / kXcds;
-        at = w * a.total / a.workgroups;
-        end = (w + 1) * a.total / a.workgroups;
-    } else {
-        // segment blockIdx.x: found like a tile below, its run is all of it
-        const int64_t seg = blockIdx.x;
-        const int per_seq = c.kv_heads * a.row_tiles;
-        const int b = (int)(seg / per_seq), rest = (int)(seg % per_seq);
-        at = a.begin[b] + (int64_t)(rest / a.row_tiles) * a.head_tiles[b];
-        for (int rt = 0; rt < rest % a.row_tiles; ++rt) at += tiles_of(a.prior[b], a.queries, a.tile_queries, rt);
-        end = at + tiles_of(a.prior[b], a.queries, a.tile_queries, rest % a.row_tiles);
+    if (!a.split) {
+        const int rt = (int)(blockIdx.x % a.row_tiles), rest = (int)(blockIdx.x / a.row_tiles);
+        const int b = rest / c.kv_heads;
+        const int tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, rt);
+        run(b, rest % c.kv_heads, rt, 0, tiles, tiles, 0);
+        return;
     }
+    const int w = a.workgroups % kXcds ? (int)blockIdx.x
+                                       : (int)(blockIdx.x % kXcds) * (a.workgroups / kXcds) + (int)(blockIdx.x / kXcds);
+    int at = first_tile(a, w);
+    const int end = first_tile(a, w + 1);
     int b = 0;
     for (int hi = a.batch - 1; b < hi;) {
         const int mid = (b + hi + 1) >> 1;
         if (a.begin[mid] <= at) b = mid;
         else hi = mid - 1;
     }
-    int head = (int)((at - a.begin[b]) / a.head_tiles[b]), rt = 0;
-    int64_t seg_begin = a.begin[b] + (int64_t)head * a.head_tiles[b];
+    int head = (at - a.begin[b]) / a.head_tiles[b], rt = 0;
+    int seg_begin = a.begin[b] + head * a.head_tiles[b];
     int tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, 0);
     while (seg_begin + tiles <= at) {
         seg_begin += tiles;
         tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, ++rt);
     }
+    Part begun = {};
     for (bool again = false; at < end; again = true) {
         if (again) __syncthreads();  // the LDS of the part before is free
-        const int tile = (int)(at - seg_begin), tile_end = (int)min((int64_t)tiles, end - seg_begin);
-        run(b, head, rt, tile, tile_end, seg_begin, tiles);
+        const int tile = at - seg_begin, tile_end = min(tiles, end - seg_begin);
+        if (tile == 0 && tile_end < tiles) begun = Part{b, head, rt, owner_of(a, seg_begin + tiles - 1) - w + 1};
+        run(b, head, rt, tile, tile_end, tiles, w);
         at = seg_begin + tile_end;
         seg_begin += tiles;
         if (++rt == a.row_tiles) {
@@ -517,13 +488,70 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
         }
         tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, rt);
     }
+    if (tid == 0) a.parts[w] = begun;
+}
+
+// Merges the parts of a segment in the order of its keys: a workgroup per
+// wavefront's 32 rows, its wavefronts 32 dims each.  (The workgroup that ends
+// last, alone with all rows, took 5 us per part of 133 KB.)
+template <int MT>
+__global__ __launch_bounds__(64 * MT) void merge_kernel(PrefillArgs a) {
+    constexpr int PAIRS = MT * 8 + 1;
+    constexpr int K = 4;  // parts whose loads go out together
+    const int wave = (int)(blockIdx.x % kWaves), w0 = (int)(blockIdx.x / kWaves);
+    const Part seg = a.parts[w0];
+    const int b = seg.b, head = seg.head, rt = seg.rt, parts = seg.count;
+    if (parts == 0) return;
+    const int lane = threadIdx.x & 63, mt = threadIdx.x >> 6;
+    const int group = a.q_heads / a.cache.kv_heads, d = a.cache.head_dim;
+    const int r = wave * 32 + (lane & 31), query = rt * a.tile_queries + r / group;
+    if (r >= a.tile_queries * group || query >= a.queries) return;
+    float m = -__FLT_MAX__, l = 0.0f;
+    float2 o[8] = {};
+    for (int j = 0; j < parts; j += K) {
+        float2 x[K][8], ml[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int p = min(j + k, parts - 1);
+            const float2 *from = part_at(a, w0 + p, p == 0, wave, PAIRS) + lane;
+            ml[k] = from[MT * 8 * 64];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[k][i] = from[(mt * 8 + i) * 64];
+        }
+        float m_new = m;
+#pragma unroll
+        for (int k = 0; k < K; ++k) m_new = fmaxf(m_new, ml[k].x);
+        const float keep = __builtin_amdgcn_exp2f(m - m_new);
+        m = m_new;
+        l *= keep;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = make_float2(o[i].x * keep, o[i].y * keep);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (j + k >= parts) continue;
+            const float w = __builtin_amdgcn_exp2f(ml[k].x - m);
+            l = fmaf(ml[k].y, w, l);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = make_float2(fmaf(x[k][i].x, w, o[i].x), fmaf(x[k][i].y, w, o[i].y));
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t *op = a.out + (((int64_t)b * a.queries + query) * a.q_heads + head * group + r % group) * d + mt * 32 +
+                   (lane >> 5) * 4;
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+        uint2 w;
+        w.x = pack_bf16x2(o[2 * i4].x * inv, o[2 * i4].y * inv);
+        w.y = pack_bf16x2(o[2 * i4 + 1].x * inv, o[2 * i4 + 1].y * inv);
+        if (mt * 32 + i4 * 8 < d) *reinterpret_cast<uint2 *>(op + i4 * 8) = w;
+    }
 }
 
 struct Shape {
     int tile_queries, row_tiles;
-    int64_t total, workgroups, segments;
-    int64_t begin[kKv8Batch + 1];
-    int64_t head_tiles[kKv8Batch];
+    int64_t total, segments;
+    int workgroups;
+    int64_t begin[kKv8Batch + 1], head_tiles[kKv8Batch];
 };
 Shape shape_of(const Kv8AttentionLaunch &l) {
     Shape s{};
@@ -537,7 +565,7 @@ Shape shape_of(const Kv8AttentionLaunch &l) {
         s.begin[b + 1] = s.begin[b] + tiles * l.cache.kv_heads;
     }
     s.total = s.begin[l.batch];
-    s.workgroups = std::min<int64_t>(s.total, kCus);
+    s.workgroups = (int)std::min<int64_t>(s.total, kCus);
     return s;
 }
 
@@ -557,12 +585,19 @@ bool kv8_prefill_supported(const Kv8AttentionLaunch &l) {
     return l.cache.head_dim <= 128 && group <= kRows && rows > 64;
 }
 
+namespace {
+size_t part_bytes(const Kv8AttentionLaunch &l, const Shape &s) {
+    const size_t pairs = (l.cache.head_dim <= 64 ? 2 : 4) * 8 + 1;
+    return (size_t)(2 * s.workgroups) * kWaves * pairs * 64 * sizeof(float2);
+}
+}  // namespace
+
 Kv8AttentionPlan kv8_prefill_plan(const Kv8AttentionLaunch &l) {
     const Shape s = shape_of(l);
     Kv8AttentionPlan p{};
-    const int pairs = (l.cache.head_dim <= 64 ? 2 : 4) * 8 + 1;
-    p.partial_bytes = (size_t)(2 * s.workgroups) * kWaves * pairs * 64 * 2 * sizeof(float);
-    p.counters = (size_t)s.segments;
+    if (s.total > INT32_MAX / 2) return p;  // positions of tiles are 32 bits
+    p.split = true;
+    p.partial_bytes = part_bytes(l, s) + s.workgroups * sizeof(Part);
     return p;
 }
 
@@ -571,17 +606,19 @@ hipError_t launch_kv8_prefill(const Kv8AttentionLaunch &l, hipStream_t stream) {
     PrefillArgs a{};
     a.cache = l.cache;
     a.q = l.q; a.out = l.out;
-    a.partial = l.partial; a.counters = l.counters;
+    a.partial = reinterpret_cast<float2 *>(l.partial);
     a.batch = l.batch; a.queries = l.queries; a.q_heads = l.q_heads;
     a.tile_queries = s.tile_queries;
     a.row_tiles = s.row_tiles;
     a.scale_log2e = l.scale * kLog2e;
     a.split = l.split;
-    a.total = s.total;
     a.workgroups = s.workgroups;
+    a.share = (int)(s.total / s.workgroups);
+    a.extra = (int)(s.total % s.workgroups);
+    if (l.split) a.parts = reinterpret_cast<Part *>(reinterpret_cast<char *>(l.partial) + part_bytes(l, s));
     for (int b = 0; b < l.batch; ++b) {
-        a.begin[b + 1] = s.begin[b + 1];
-        a.head_tiles[b] = s.head_tiles[b];
+        a.begin[b + 1] = (int)s.begin[b + 1];  // split launches only
+        a.head_tiles[b] = (int)s.head_tiles[b];
         a.prior[b] = l.len[b] - l.queries;
     }
     const unsigned grid = (unsigned)(l.split ? s.workgroups : s.segments);
@@ -591,6 +628,10 @@ hipError_t launch_kv8_prefill(const Kv8AttentionLaunch &l, hipStream_t stream) {
     if (l.cache.format == kFormatE4m3) { MSLIM_KV8_PREFILL(kFormatE4m3); }
     else { MSLIM_KV8_PREFILL(kFormatInt8); }
 #undef MSLIM_KV8_PREFILL
+    if (hipError_t err = hipGetLastError(); err != hipSuccess || !l.split) return err;
+    const dim3 merge((unsigned)(s.workgroups * kWaves));
+    if (l.cache.head_dim <= 64) hipLaunchKernelGGL((merge_kernel<2>), merge, dim3(128), 0, stream, a);
+    else hipLaunchKernelGGL((merge_kernel<4>), merge, dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
