@@ -1203,6 +1203,44 @@ static bool kv8_overlaps(const mslim_attn_kv8_cache *cache, const void *p) {
     return p == cache->k_pool || p == cache->v_pool || p == cache->scales;
 }
 
+// Turns per position of every rotary pair, in 64 bits: the inverse frequency
+// theta^(-2f / head_dim), scaled by parts of the wavelength range where asked,
+// over 2 pi.  The last ones are kept per thread: a decode step makes the same
+// call for every layer, and 64 powers take longer than its launch.
+static const mslim::Kv8Turns &kv8_turns(int head_dim, float theta, int llama3, float factor, float low, float high,
+                                        float original_max) {
+    struct Key {
+        int head_dim, llama3;
+        float theta, factor, low, high, original_max;
+    };
+    static thread_local Key last{};
+    static thread_local mslim::Kv8Turns turns;
+    Key key{head_dim, llama3 != 0, theta, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (llama3) {
+        key.factor = factor;
+        key.low = low;
+        key.high = high;
+        key.original_max = original_max;
+    }
+    if (std::memcmp(&key, &last, sizeof key) == 0) return turns;
+    const double two_pi = 6.28318530717958647692528676655900577;
+    for (int f = 0; f < head_dim / 2; ++f) {
+        double inv = std::pow((double)theta, -2.0 * f / head_dim);
+        if (llama3) {
+            const double wavelength = two_pi / inv;
+            if (wavelength > (double)original_max / low) {
+                inv /= factor;
+            } else if (wavelength >= (double)original_max / high) {
+                const double smooth = (original_max / wavelength - low) / ((double)high - low);
+                inv = (1.0 - smooth) * inv / factor + smooth * inv;
+            }
+        }
+        turns.turn[f] = inv / two_pi;
+    }
+    last = key;
+    return turns;
+}
+
 int mslim_attn_rope_append_kv8(void *ctx, const mslim_attn_kv8_cache *cache, const void *q, const void *k,
                                const void *v, void *q_out, int batch, int tokens, const int32_t *positions,
                                int q_heads, float theta, int llama3_scaling, float factor,
@@ -1226,24 +1264,8 @@ int mslim_attn_rope_append_kv8(void *ctx, const mslim_attn_kv8_cache *cache, con
         if (llama3_scaling && (!(factor > 0.0f) || !(high_freq_factor > low_freq_factor) ||
                                !(low_freq_factor > 0.0f) || !(original_max_position > 0.0f)))
             return fail("invalid llama3 RoPE scaling parameters");
-        // Turns per position of every pair, in 64 bits: the inverse
-        // frequency theta^(-2f / head_dim), scaled by parts of the wavelength
-        // range where asked, over 2 pi.
-        const double two_pi = 6.28318530717958647692528676655900577;
-        for (int f = 0; f < cache->head_dim / 2; ++f) {
-            double inv = std::pow((double)theta, -2.0 * f / cache->head_dim);
-            if (llama3_scaling) {
-                const double wavelength = two_pi / inv;
-                if (wavelength > (double)original_max_position / low_freq_factor) {
-                    inv /= factor;
-                } else if (wavelength >= (double)original_max_position / high_freq_factor) {
-                    const double smooth = (original_max_position / wavelength - low_freq_factor) /
-                                          ((double)high_freq_factor - low_freq_factor);
-                    inv = (1.0 - smooth) * inv / factor + smooth * inv;
-                }
-            }
-            l.turns.turn[f] = inv / two_pi;
-        }
+        l.turns = kv8_turns(cache->head_dim, theta, llama3_scaling, factor, low_freq_factor, high_freq_factor,
+                            original_max_position);
     }
     l.q = static_cast<const uint16_t *>(q);
     l.k = static_cast<const uint16_t *>(k);

@@ -81,12 +81,14 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 
 // c and s of a rotary pair: the angle is position * turn periods in 64 bits,
 // reduced to half a period there, so positions keep their full accuracy
-// however far they are; the functions and the rotation are in 32.
+// however far they are.  The functions are rounded to 32 bits once: the f32
+// ones, a unit off now and then, moved one byte in 10^6 that a rounding apart
+// from them does not.
 __device__ __forceinline__ float2 turn_cs(int64_t position, double turn) {
     const double t = (double)position * turn;
-    float s, c;
-    sincospif((float)(2.0 * (t - rint(t))), &s, &c);
-    return make_float2(c, s);
+    double s, c;
+    sincospi(2.0 * (t - rint(t)), &s, &c);
+    return make_float2((float)c, (float)s);
 }
 
 // Index of the 16-token block that holds token t (>= 0) of a sequence, or -1

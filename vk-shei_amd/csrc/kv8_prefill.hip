@@ -22,10 +22,13 @@ constexpr float kLazyBound = 256.0f;
 
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
-// A segment that workgroup w is the first but not the only one to take, for
-// the merge: `count` parts, by w, w + 1, ...; 0 where there is none.
+// How the segments of a launch are shared out.
+constexpr int kWhole = 0, kPieces = 1, kRuns = 2;
+
+// A segment of several parts, for the merge: workgroups w0, w0 + 1, ... took
+// `count` parts; 0 where there is nothing to merge.
 struct Part {
-    int b, head, rt, count;
+    int b, head, rt, w0, count;
 };
 
 struct PrefillArgs {
@@ -33,19 +36,20 @@ struct PrefillArgs {
     const uint16_t *q;
     uint16_t *out;
     float2 *partial;  // [2 * workgroups][wavefront][pair][64]: O, then (m, l)
-    Part *parts;      // [workgroups]
+    Part *parts;      // kPieces: [segments], kRuns: [workgroups]
     int batch, queries, q_heads;
     int tile_queries;  // queries of a row tile: kRows / group
     int row_tiles;
     float scale_log2e;
-    // Segments (sequence, kv head, row tile) laid end to end.  Workgroup w of
-    // a split launch takes `share` tiles of them (one more for the first
-    // `extra` workgroups) from first_tile(w) on, an unsplit one has a
-    // workgroup per segment.
-    bool split;
-    int share, extra, workgroups;
-    int begin[kKv8Batch + 1];   // first tile of each sequence
-    int head_tiles[kKv8Batch];  // tiles of one kv head of each sequence
+    // Segments (sequence, kv head, row tile) laid end to end, by MODE:
+    //   kWhole   a workgroup per segment;
+    //   kPieces  a workgroup per piece of a segment, of `quota` tiles at most;
+    //   kRuns    workgroup w takes `share` tiles (one more for the first
+    //            `extra` workgroups) from first_tile(w) on.
+    int mode;
+    int quota, share, extra, workgroups;
+    int begin[kKv8Batch + 1];   // first tile (kPieces: piece) of each sequence
+    int per_head[kKv8Batch];    // tiles (kPieces: pieces) of one kv head of each sequence
     int prior[kKv8Batch];
 };
 
@@ -447,7 +451,7 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
 
     // Workgroup -> run of tiles: XCD x (workgroups x, x + 8, ...) takes a
     // contiguous eighth of all, so the kv heads that it reads stay in its L2.
-    if (!a.split) {
+    if (a.mode == kWhole) {
         const int rt = (int)(blockIdx.x % a.row_tiles), rest = (int)(blockIdx.x / a.row_tiles);
         const int b = rest / c.kv_heads;
         const int tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, rt);
@@ -456,17 +460,30 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
     }
     const int w = a.workgroups % kXcds ? (int)blockIdx.x
                                        : (int)(blockIdx.x % kXcds) * (a.workgroups / kXcds) + (int)(blockIdx.x / kXcds);
-    int at = first_tile(a, w);
-    const int end = first_tile(a, w + 1);
+    int at = a.mode == kPieces ? w : first_tile(a, w);
     int b = 0;
     for (int hi = a.batch - 1; b < hi;) {
         const int mid = (b + hi + 1) >> 1;
         if (a.begin[mid] <= at) b = mid;
         else hi = mid - 1;
     }
-    int head = (at - a.begin[b]) / a.head_tiles[b], rt = 0;
-    int seg_begin = a.begin[b] + head * a.head_tiles[b];
+    int head = (at - a.begin[b]) / a.per_head[b], rt = 0;
+    int seg_begin = a.begin[b] + head * a.per_head[b];
     int tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, 0);
+    if (a.mode == kPieces) {
+        int pieces = (tiles + a.quota - 1) / a.quota;
+        while (seg_begin + pieces <= at) {
+            seg_begin += pieces;
+            tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, ++rt);
+            pieces = (tiles + a.quota - 1) / a.quota;
+        }
+        const int i = at - seg_begin;
+        run(b, head, rt, i * tiles / pieces, (i + 1) * tiles / pieces, tiles, w);
+        if (tid == 0 && i == 0)
+            a.parts[(b * c.kv_heads + head) * a.row_tiles + rt] = Part{b, head, rt, w, pieces > 1 ? pieces : 0};
+        return;
+    }
+    const int end = first_tile(a, w + 1);
     while (seg_begin + tiles <= at) {
         seg_begin += tiles;
         tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, ++rt);
@@ -475,7 +492,7 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
     for (bool again = false; at < end; again = true) {
         if (again) __syncthreads();  // the LDS of the part before is free
         const int tile = at - seg_begin, tile_end = min(tiles, end - seg_begin);
-        if (tile == 0 && tile_end < tiles) begun = Part{b, head, rt, owner_of(a, seg_begin + tiles - 1) - w + 1};
+        if (tile == 0 && tile_end < tiles) begun = Part{b, head, rt, w, owner_of(a, seg_begin + tiles - 1) - w + 1};
         run(b, head, rt, tile, tile_end, tiles, w);
         at = seg_begin + tile_end;
         seg_begin += tiles;
@@ -491,18 +508,18 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
     if (tid == 0) a.parts[w] = begun;
 }
 
-// Merges the parts of a segment in the order of its keys: a workgroup per
-// wavefront's 32 rows, its wavefronts 32 dims each.  (The workgroup that ends
-// last, alone with all rows, took 5 us per part of 133 KB.)
+// Merges the parts of a segment in the order of its keys: a wavefront per 32
+// rows and 32 dims.  (The workgroup that ends last, alone with all rows, took
+// 5 us per part of 133 KB.)
 template <int MT>
-__global__ __launch_bounds__(64 * MT) void merge_kernel(PrefillArgs a) {
+__global__ __launch_bounds__(64) void merge_kernel(PrefillArgs a) {
     constexpr int PAIRS = MT * 8 + 1;
     constexpr int K = 4;  // parts whose loads go out together
-    const int wave = (int)(blockIdx.x % kWaves), w0 = (int)(blockIdx.x / kWaves);
-    const Part seg = a.parts[w0];
-    const int b = seg.b, head = seg.head, rt = seg.rt, parts = seg.count;
+    const int mt = (int)(blockIdx.x % MT), wave = (int)(blockIdx.x / MT % kWaves);
+    const Part seg = a.parts[blockIdx.x / MT / kWaves];
+    const int b = seg.b, head = seg.head, rt = seg.rt, w0 = seg.w0, parts = seg.count;
     if (parts == 0) return;
-    const int lane = threadIdx.x & 63, mt = threadIdx.x >> 6;
+    const int lane = threadIdx.x;
     const int group = a.q_heads / a.cache.kv_heads, d = a.cache.head_dim;
     const int r = wave * 32 + (lane & 31), query = rt * a.tile_queries + r / group;
     if (r >= a.tile_queries * group || query >= a.queries) return;
@@ -550,22 +567,53 @@ __global__ __launch_bounds__(64 * MT) void merge_kernel(PrefillArgs a) {
 struct Shape {
     int tile_queries, row_tiles;
     int64_t total, segments;
-    int workgroups;
-    int64_t begin[kKv8Batch + 1], head_tiles[kKv8Batch];
+    int mode, quota, workgroups;
+    int64_t begin[kKv8Batch + 1], per_head[kKv8Batch];
 };
 Shape shape_of(const Kv8AttentionLaunch &l) {
     Shape s{};
     s.tile_queries = kRows / (l.q_heads / l.cache.kv_heads);
     s.row_tiles = (l.queries + s.tile_queries - 1) / s.tile_queries;
     s.segments = (int64_t)l.batch * l.cache.kv_heads * s.row_tiles;
-    for (int b = 0; b < l.batch; ++b) {
-        int64_t tiles = 0;
-        for (int rt = 0; rt < s.row_tiles; ++rt) tiles += tiles_of(l.len[b] - l.queries, l.queries, s.tile_queries, rt);
-        s.head_tiles[b] = tiles;
-        s.begin[b + 1] = s.begin[b] + tiles * l.cache.kv_heads;
+    // tiles (pieces of at most `quota`, where given) of all segments
+    auto lay = [&](int quota) {
+        for (int b = 0; b < l.batch; ++b) {
+            int64_t n = 0;
+            for (int rt = 0; rt < s.row_tiles; ++rt) {
+                const int tiles = tiles_of(l.len[b] - l.queries, l.queries, s.tile_queries, rt);
+                n += quota ? (tiles + quota - 1) / quota : tiles;
+            }
+            s.per_head[b] = n;
+            s.begin[b + 1] = s.begin[b] + n * l.cache.kv_heads;
+        }
+        return s.begin[l.batch];
+    };
+    s.total = lay(0);
+    if (s.segments <= kCus) {
+        // The size of a piece with the shortest call, of those that leave no
+        // more pieces than CUs: a tile takes a workgroup 2 us, a part 0.06 us
+        // of the device's bandwidth (133 KB written and read) and 0.2 us in
+        // the merge's chain.
+        s.mode = kPieces;
+        int longest = 1;
+        for (int b = 0; b < l.batch; ++b)
+            longest = std::max(longest, tiles_of(l.len[b] - l.queries, l.queries, s.tile_queries, s.row_tiles - 1));
+        double best = 0.0;
+        for (int q = (int)std::max<int64_t>(1, s.total / kCus); q <= longest; q += 1 + q / 16) {
+            const int64_t pieces = lay(q);
+            if (pieces > kCus) continue;
+            const double cost = 2.0 * q + 0.06 * (double)pieces + 0.2 * ((longest + q - 1) / q);
+            if (!s.quota || cost < best) {
+                best = cost;
+                s.quota = q;
+            }
+        }
+        if (!s.quota) s.quota = longest;
+        s.workgroups = (int)lay(s.quota);
+    } else {
+        s.mode = s.total > INT32_MAX / 2 ? kWhole : kRuns;  // positions of tiles are 32 bits
+        s.workgroups = (int)std::min<int64_t>(s.total, kCus);
     }
-    s.total = s.begin[l.batch];
-    s.workgroups = (int)std::min<int64_t>(s.total, kCus);
     return s;
 }
 
@@ -590,14 +638,15 @@ size_t part_bytes(const Kv8AttentionLaunch &l, const Shape &s) {
     const size_t pairs = (l.cache.head_dim <= 64 ? 2 : 4) * 8 + 1;
     return (size_t)(2 * s.workgroups) * kWaves * pairs * 64 * sizeof(float2);
 }
+size_t merges(const Shape &s) { return s.mode == kPieces ? (size_t)s.segments : (size_t)s.workgroups; }
 }  // namespace
 
 Kv8AttentionPlan kv8_prefill_plan(const Kv8AttentionLaunch &l) {
     const Shape s = shape_of(l);
     Kv8AttentionPlan p{};
-    if (s.total > INT32_MAX / 2) return p;  // positions of tiles are 32 bits
+    if (s.mode == kWhole) return p;
     p.split = true;
-    p.partial_bytes = part_bytes(l, s) + s.workgroups * sizeof(Part);
+    p.partial_bytes = part_bytes(l, s) + merges(s) * sizeof(Part);
     return p;
 }
 
@@ -611,14 +660,15 @@ hipError_t launch_kv8_prefill(const Kv8AttentionLaunch &l, hipStream_t stream) {
     a.tile_queries = s.tile_queries;
     a.row_tiles = s.row_tiles;
     a.scale_log2e = l.scale * kLog2e;
-    a.split = l.split;
+    a.mode = l.split ? s.mode : kWhole;
+    a.quota = s.quota;
     a.workgroups = s.workgroups;
     a.share = (int)(s.total / s.workgroups);
     a.extra = (int)(s.total % s.workgroups);
     if (l.split) a.parts = reinterpret_cast<Part *>(reinterpret_cast<char *>(l.partial) + part_bytes(l, s));
     for (int b = 0; b < l.batch; ++b) {
         a.begin[b + 1] = (int)s.begin[b + 1];  // split launches only
-        a.head_tiles[b] = (int)s.head_tiles[b];
+        a.per_head[b] = (int)s.per_head[b];
         a.prior[b] = l.len[b] - l.queries;
     }
     const unsigned grid = (unsigned)(l.split ? s.workgroups : s.segments);
@@ -629,9 +679,10 @@ hipError_t launch_kv8_prefill(const Kv8AttentionLaunch &l, hipStream_t stream) {
     else { MSLIM_KV8_PREFILL(kFormatInt8); }
 #undef MSLIM_KV8_PREFILL
     if (hipError_t err = hipGetLastError(); err != hipSuccess || !l.split) return err;
-    const dim3 merge((unsigned)(s.workgroups * kWaves));
-    if (l.cache.head_dim <= 64) hipLaunchKernelGGL((merge_kernel<2>), merge, dim3(128), 0, stream, a);
-    else hipLaunchKernelGGL((merge_kernel<4>), merge, dim3(256), 0, stream, a);
+    if (s.mode == kPieces && s.workgroups == s.segments) return hipSuccess;  // nothing was split
+    const unsigned merge = (unsigned)(merges(s) * kWaves);
+    if (l.cache.head_dim <= 64) hipLaunchKernelGGL((merge_kernel<2>), dim3(merge * 2), dim3(64), 0, stream, a);
+    else hipLaunchKernelGGL((merge_kernel<4>), dim3(merge * 4), dim3(64), 0, stream, a);
     return hipGetLastError();
 }
 
