@@ -92,9 +92,11 @@ __device__ __forceinline__ float2 turn_cs(int64_t position, double turn) {
 }
 
 // Index of the 16-token block that holds token t (>= 0) of a sequence, or -1
-// where the table names no page of the pool.
-__device__ __forceinline__ int64_t block_of(const Kv8Cache &c, int b, int head, int64_t t) {
-    const int64_t page = c.table[(int64_t)b * c.pages_per_seq + (t >> c.shift)];
+// where the table names no page of the pool.  scalar: the same for the whole
+// wavefront.
+__device__ __forceinline__ int64_t block_of(const Kv8Cache &c, int b, int head, int64_t t, bool scalar = false) {
+    const int64_t page = scalar ? scalar_page(c.table + (int64_t)b * c.pages_per_seq + (t >> c.shift))
+                                : c.table[(int64_t)b * c.pages_per_seq + (t >> c.shift)];
     if (page < 0 || page >= c.pool_pages) return -1;
     return ((page * c.kv_heads + head) << (c.shift - 4)) + ((t & ((1 << c.shift) - 1)) >> 4);
 }
@@ -107,7 +109,7 @@ struct AppendArgs {
     int batch, tokens, q_heads;
     int blocks;     // 16-token blocks that `tokens` rows can reach
     int kv_groups;  // workgroups of a block: four kv heads each
-    int64_t kv_workgroups;
+    uint32_t kv_workgroups;
     Kv8Turns turns;
 };
 
@@ -135,17 +137,21 @@ __device__ __forceinline__ void rotate8(float (&x)[8], float (&p)[8], const floa
 // kv head); the others rotate a row of Q each.  The rows of a block that are
 // not new and lie before the new ones are read only where the block's scale
 // grows; the rows behind keep their bytes.  NI: units of 8 pairs of a lane.
-template <int FMT, int NI, bool ROTATE>
+// DIM: head_dim where it is 64, 128 or 256, else 0: a step of one token is a
+// chain of a few loads and sums, in which the divisions by a head_dim known at
+// run time alone took 1.6 of 6.2 us.
+template <int FMT, int NI, bool ROTATE, int DIM>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     __shared__ float2 cs_lds[16 * 16 * NI * 2];  // [16 rows][half <= 32 * NI]
     const Kv8Cache &c = a.cache;
-    const int d = c.head_dim, half = d / 2;
+    const int d = DIM ? DIM : c.head_dim, half = d / 2;
     const int hc = half / 8;  // units per head row
     const int tid = threadIdx.x;
-    if ((int64_t)blockIdx.x >= a.kv_workgroups) {
+    if (blockIdx.x >= a.kv_workgroups) {
         if constexpr (ROTATE) {
-            const int64_t row = blockIdx.x - a.kv_workgroups;  // batch * tokens
-            const int64_t position = (int64_t)a.positions[row / a.tokens] + row % a.tokens;
+            const uint32_t r = blockIdx.x - a.kv_workgroups;  // of batch * tokens
+            const int64_t row = r;
+            const int64_t position = (int64_t)scalar_page(a.positions + r / (uint32_t)a.tokens) + r % (uint32_t)a.tokens;
             for (int f = tid; f < half; f += 256) cs_lds[f] = turn_cs(position, a.turns.turn[f]);
             __syncthreads();
             const uint16_t *src = a.q + row * a.q_heads * d;
@@ -168,28 +174,57 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     }
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int group = (int)(blockIdx.x % a.kv_groups);
-    const int64_t bj = blockIdx.x / a.kv_groups;
-    const int b = (int)(bj / a.blocks);
-    const int64_t pos = a.positions[b];
-    const int64_t base = ((pos >> 4) + bj % a.blocks) * 16;  // first token of the block
+    const int group = (int)(blockIdx.x % (uint32_t)a.kv_groups);
+    const uint32_t bj = blockIdx.x / (uint32_t)a.kv_groups;
+    const int b = (int)(bj / (uint32_t)a.blocks);
+    const int64_t pos = scalar_page(a.positions + b);
+    const int64_t base = ((pos >> 4) + bj % (uint32_t)a.blocks) * 16;  // first token of the block
     const int64_t capacity = (int64_t)c.pages_per_seq << c.shift;
     const int64_t lo64 = max(max(pos, base), (int64_t)0);
     const int64_t hi64 = min(min(pos + a.tokens, base + 16), capacity);
     if (base < 0 || lo64 >= hi64) return;  // uniform over the workgroup
     const int lo = (int)(lo64 - base), n = (int)(hi64 - lo64);
     const int64_t row0 = (int64_t)b * a.tokens + (lo64 - pos);  // of k and v
+    const int head = group * 4 + wave;
+    const bool active = head < c.kv_heads;
+    const int64_t block = active ? block_of(c, b, head, base, true) : -1;
+    float2 *scale_at = reinterpret_cast<float2 *>(c.scales) + max(block, (int64_t)0);
+
+    // All loads go out before the cos and sin are computed: a step of one
+    // token is a chain of them.  K: a lane's units are (row, 8 pairs); V:
+    // (four tokens, 8 dims).
+    constexpr int NV = (NI + 1) / 2;
+    const int dc = d / 8;
+    uint4 kx[NI], kp[NI], rows[NV][4];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int u = lane + 64 * i;
+        if (active && u < n * hc) {
+            const uint16_t *src = a.k + ((row0 + u / hc) * c.kv_heads + head) * d + u % hc * 8;
+            kx[i] = *reinterpret_cast<const uint4 *>(src);
+            kp[i] = *reinterpret_cast<const uint4 *>(src + half);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int u = lane + 64 * i;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int r = u / dc * 4 + t - lo;  // among the new rows
+            rows[i][t] = make_uint4(0, 0, 0, 0);
+            if (active && u < 4 * dc && r >= 0 && r < n)
+                rows[i][t] = *reinterpret_cast<const uint4 *>(a.v + ((row0 + r) * c.kv_heads + head) * d + u % dc * 8);
+        }
+    }
+    float2 old = make_float2(0.0f, 0.0f);
+    if (lo > 0) old = scalar_scales(reinterpret_cast<const float *>(scale_at));  // this wavefront alone writes it
     if constexpr (ROTATE) {
         for (int u = tid; u < n * half; u += 256)
             cs_lds[u] = turn_cs(lo64 + u / half, a.turns.turn[u % half]);
         __syncthreads();
     }
-    const int head = group * 4 + wave;
-    if (head >= c.kv_heads) return;
-    const int64_t block = block_of(c, b, head, base);
     if (block < 0) return;
 
-    // K: lane's units are (row, 8 pairs).
     uint8_t *kb = c.k + block * 16 * d;
     float x[NI][8], p[NI][8];
     uint32_t amax = 0;
@@ -197,19 +232,14 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     for (int i = 0; i < NI; ++i) {
         const int u = lane + 64 * i;
         if (u < n * hc) {
-            const int r = u / hc, at = u % hc * 8;
-            const uint16_t *src = a.k + ((row0 + r) * c.kv_heads + head) * d + at;
-            unpack8(*reinterpret_cast<const uint4 *>(src), x[i]);
-            unpack8(*reinterpret_cast<const uint4 *>(src + half), p[i]);
-            if constexpr (ROTATE) rotate8(x[i], p[i], cs_lds + r * half + at);
+            unpack8(kx[i], x[i]);
+            unpack8(kp[i], p[i]);
+            if constexpr (ROTATE) rotate8(x[i], p[i], cs_lds + u / hc * half + u % hc * 8);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 amax = max(amax, max(__float_as_uint(x[i][j]) & 0x7fffffffu, __float_as_uint(p[i][j]) & 0x7fffffffu));
         }
     }
-    float2 *scale_at = reinterpret_cast<float2 *>(c.scales) + block;
-    float2 old = make_float2(0.0f, 0.0f);
-    if (lo > 0) old = *scale_at;
     // The scale that covers old rows and new ones; NaN on either side stays.
     auto cover = [&](uint32_t top, float before) {
         const float fresh = scale_of<FMT>(top);
@@ -241,26 +271,16 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         }
     }
 
-    // V: lane's units are (four tokens, 8 dims).
-    constexpr int NV = (NI + 1) / 2;
     uint8_t *vb = c.v + block * 16 * d;
-    const int dc = d / 8;
-    uint4 rows[NV][4];
     amax = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int u = lane + 64 * i;
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const int r = u / dc * 4 + t - lo;  // among the new rows
-            rows[i][t] = make_uint4(0, 0, 0, 0);
-            if (u < 4 * dc && r >= 0 && r < n)
-                rows[i][t] = *reinterpret_cast<const uint4 *>(a.v + ((row0 + r) * c.kv_heads + head) * d + u % dc * 8);
             const uint32_t w[4] = {rows[i][t].x, rows[i][t].y, rows[i][t].z, rows[i][t].w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) amax = max(amax, max(w[j] << 16 & 0x7fffffffu, w[j] & 0x7fff0000u));
         }
-    }
     const float vs = cover(wave_max(amax), old.y);
     const float vi = inverse(vs);
     const bool grown = lo > 0 && vs > old.y;
@@ -875,12 +895,15 @@ void launch_attention(const AttentionArgs &a, const Shape &s, unsigned grid, hip
 template <int FMT>
 void launch_append(const AppendArgs &a, bool rotate, unsigned grid, hipStream_t stream) {
     const int d = a.cache.head_dim;
-#define MSLIM_KV8_APPEND(NI)                                                                                  \
-    if (rotate) hipLaunchKernelGGL((append_kernel<FMT, NI, true>), dim3(grid), dim3(256), 0, stream, a);     \
-    else hipLaunchKernelGGL((append_kernel<FMT, NI, false>), dim3(grid), dim3(256), 0, stream, a)
-    if (d <= 64) { MSLIM_KV8_APPEND(1); }
-    else if (d <= 128) { MSLIM_KV8_APPEND(2); }
-    else { MSLIM_KV8_APPEND(4); }
+#define MSLIM_KV8_APPEND(NI, DIM)                                                                                  \
+    if (rotate) hipLaunchKernelGGL((append_kernel<FMT, NI, true, DIM>), dim3(grid), dim3(256), 0, stream, a);     \
+    else hipLaunchKernelGGL((append_kernel<FMT, NI, false, DIM>), dim3(grid), dim3(256), 0, stream, a)
+    if (d == 64) { MSLIM_KV8_APPEND(1, 64); }
+    else if (d == 128) { MSLIM_KV8_APPEND(2, 128); }
+    else if (d == 256) { MSLIM_KV8_APPEND(4, 256); }
+    else if (d < 64) { MSLIM_KV8_APPEND(1, 0); }
+    else if (d < 128) { MSLIM_KV8_APPEND(2, 0); }
+    else { MSLIM_KV8_APPEND(4, 0); }
 #undef MSLIM_KV8_APPEND
 }
 
@@ -905,7 +928,7 @@ hipError_t launch_kv8_append(const Kv8AppendLaunch &l, hipStream_t stream) {
     a.batch = l.batch; a.tokens = l.tokens; a.q_heads = l.q_heads;
     a.blocks = append_blocks(l);
     a.kv_groups = append_groups(l);
-    a.kv_workgroups = (int64_t)l.batch * a.blocks * a.kv_groups;
+    a.kv_workgroups = (uint32_t)((int64_t)l.batch * a.blocks * a.kv_groups);
     a.turns = l.turns;
     const unsigned grid = (unsigned)kv8_append_workgroups(l);
     if (l.cache.format == kFormatE4m3) launch_append<kFormatE4m3>(a, l.rotate, grid, stream);
