@@ -12,6 +12,7 @@ the device is not gfx950 the calls raise.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import math
 import os
@@ -134,6 +135,7 @@ class Kv8Cache(C.Structure):
         super().__init__(_ptr(k_pool), _ptr(v_pool), _ptr(scales), _ptr(page_table), pool_pages, pages_per_seq,
                          page_tokens, kv_heads, head_dim, format, 0)
         self.tensors = (k_pool, v_pool, scales, page_table)
+        self.default_scale = default_scale(head_dim) if head_dim > 0 else 0.0
 
 
 class MslimAttnError(RuntimeError):
@@ -161,7 +163,7 @@ def library() -> C.CDLL:
                              f"{LIB_PATH} is not built (run __graft_entry__.build())")
     lib = C.CDLL(LIB_PATH)
     P, I, SZ, F, I64 = C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.c_int64
-    PI32 = C.POINTER(C.c_int32)
+    PI32, PKV8 = C.POINTER(C.c_int32), C.POINTER(Kv8Cache)
     sigs = {
         "mslim_attn_last_error": (C.c_char_p, []),
         "mslim_attn_ctx_new": (P, []),
@@ -196,10 +198,10 @@ def library() -> C.CDLL:
         "mslim_attn_pages_append": (I, [P, P, P, P, I, I, I, I, I, P, P, P]),
         "mslim_attn_rope_append": (I, [P, P, P, P, P, P, P, P, I, I, I, P, I, I, I, F, I, F, F, F, F]),
         "mslim_attn_pages_gather": (I, [P, P, P, I, I, I, I64, I64, P]),
-        "mslim_attn_rope_append_kv8": (I, [P, P, P, P, P, P, I, I, P, I, F, I, F, F, F, F]),
-        "mslim_attn_pages_gather_kv8": (I, [P, P, I, I, P, P, P]),
-        "mslim_attn_decode_kv8": (I, [P, P, P, P, I, PI32, I, F]),
-        "mslim_attn_prefill_kv8": (I, [P, P, P, P, I, I, PI32, I, F]),
+        "mslim_attn_rope_append_kv8": (I, [P, PKV8, P, P, P, P, I, I, P, I, F, I, F, F, F, F]),
+        "mslim_attn_pages_gather_kv8": (I, [P, PKV8, I, I, P, P, P]),
+        "mslim_attn_decode_kv8": (I, [P, PKV8, P, P, I, P, I, F]),
+        "mslim_attn_prefill_kv8": (I, [P, PKV8, P, P, I, I, P, I, F]),
         "mslim_attn_logical_kv_sha256": (I, [P, I, I64, I, I, P, P, P, I, C.c_char_p]),
         "mslim_attn_record_frame_bytes": (I64, [I]),
         "mslim_attn_record_frames": (I, [P, P, P, I64, I, I, I, C.c_uint32, P, I, P]),
@@ -489,26 +491,29 @@ class Context:
                         original_max_position: float = 1.0) -> None:
         """Rotate Q into q_out and K, and append K and V; theta 0 appends only."""
         self._check("rope_append_kv8", self._lib.mslim_attn_rope_append_kv8(
-            self._h, C.byref(cache), _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), batch, tokens, _ptr(positions), q_heads,
-            theta, int(bool(llama3_scaling)), factor, low_freq_factor, high_freq_factor, original_max_position))
+            self._h, cache, _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), batch, tokens, _ptr(positions), q_heads,
+            theta, 1 if llama3_scaling else 0, factor, low_freq_factor, high_freq_factor, original_max_position))
 
     def pages_gather_kv8(self, cache: Kv8Cache, batch: int, tokens: int, first, k_rows, v_rows) -> None:
         """BF16 K and V rows first[b] .. first[b] + tokens - 1 (first None: from row 0)."""
         self._check("pages_gather_kv8", self._lib.mslim_attn_pages_gather_kv8(
-            self._h, C.byref(cache), batch, tokens, _ptr(first), _ptr(k_rows), _ptr(v_rows)))
+            self._h, cache, batch, tokens, _ptr(first), _ptr(k_rows), _ptr(v_rows)))
 
     def decode_kv8(self, cache: Kv8Cache, q, out, seq_lens: Sequence[int], q_heads: int,
                    scale: Optional[float] = None) -> None:
-        scale = default_scale(cache.head_dim) if scale is None else scale
+        """seq_lens: tokens of each sequence, 0 for a padded slot."""
+        lens = array.array("i", seq_lens)
         self._check("decode_kv8", self._lib.mslim_attn_decode_kv8(
-            self._h, C.byref(cache), _ptr(q), _ptr(out), len(seq_lens), _lens(seq_lens), q_heads, scale))
+            self._h, cache, _ptr(q), _ptr(out), len(lens), lens.buffer_info()[0], q_heads,
+            cache.default_scale if scale is None else scale))
 
     def prefill_kv8(self, cache: Kv8Cache, q, out, queries: int, priors: Sequence[int], q_heads: int,
                     scale: Optional[float] = None) -> None:
         """The last `queries` tokens of each sequence, already appended, over the cache."""
-        scale = default_scale(cache.head_dim) if scale is None else scale
+        lens = array.array("i", priors)
         self._check("prefill_kv8", self._lib.mslim_attn_prefill_kv8(
-            self._h, C.byref(cache), _ptr(q), _ptr(out), len(priors), queries, _lens(priors), q_heads, scale))
+            self._h, cache, _ptr(q), _ptr(out), len(lens), queries, lens.buffer_info()[0], q_heads,
+            cache.default_scale if scale is None else scale))
 
     def logical_kv_sha256(self, keys: Sequence, values: Sequence, tokens: int, kv_heads: int,
                           head_dim: int, page_tables: Optional[Sequence] = None,
