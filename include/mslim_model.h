@@ -34,6 +34,14 @@ extern "C" {
  * (the reference's invariant, mod.rs:2993-3048). */
 #define MSLIM_MODEL_KV_PAGED 0
 #define MSLIM_MODEL_KV_DENSE 1
+/* PAGED_E4M3, PAGED_INT8: pages of the 8-bit cache (mslim_attn_kv8_cache),
+ * half the bytes per token; no reference counterpart.  Queries and keys are
+ * rotated by mslim_attn_rope_append_kv8 and attention reads the 8-bit rows, in
+ * a prompt's chunks as in decode steps.  head_dim a multiple of 16.  There is
+ * no exact K/V to digest or to persist: mslim_model_logical_kv_sha256 and the
+ * ColdStore calls fail. */
+#define MSLIM_MODEL_KV_PAGED_E4M3 2
+#define MSLIM_MODEL_KV_PAGED_INT8 3
 
 /* ModelSpec fields a layer uses (src/model_config.rs:22-42) and the RoPE
  * arguments of RopeKernelConfig (src/gpu_llm/kernels.rs:15-23). */

@@ -44,7 +44,8 @@ DecoderRunner::DecoderRunner(std::shared_ptr<NativeContext> ctx, ModelSpec spec,
     ensure(max_batch_ >= 1 && max_batch_ <= kMaxSlots, "max_batch must be 1..=64");
     ensure(chunk_tokens_ >= 1 && chunk_tokens_ <= 512, "prefill chunk must be 1..=512 tokens");
     ensure(max_context_ >= 1 && max_context_ <= (1 << 24), "max_context must be 1..=16777216 tokens");
-    ensure(layout_ == KvLayout::Paged || layout_ == KvLayout::Dense, "unknown K/V layout");
+    ensure(layout_ == KvLayout::Paged || layout_ == KvLayout::Dense || eight_bit(), "unknown K/V layout");
+    ensure(!eight_bit() || spec_.head_dim % 16 == 0, "the 8-bit K/V layouts need a head_dim that is a multiple of 16");
     // The dense layout is a pool of one-token pages (token-major rows) under
     // the identity table: slot s, token t -> row s * max_context + t.
     page_tokens_ = layout_ == KvLayout::Dense ? 1 : kPageTokens;
@@ -64,7 +65,7 @@ DecoderRunner::DecoderRunner(std::shared_ptr<NativeContext> ctx, ModelSpec spec,
         // One allocation for every layer's K pages and one for V: layer l's
         // pool is pages [l * pool_pages, (l + 1) * pool_pages), so the
         // ColdStore seal and restore of a slot cover all layers per launch.
-        const size_t layer_bytes = pool_pages * page_tokens_ * kvd * 2;
+        const size_t layer_bytes = pool_pages * page_tokens_ * kvd * (eight_bit() ? 1 : 2);
         k_base_ = alloc(layer_bytes * spec_.layers);
         v_base_ = alloc(layer_bytes * spec_.layers);
         for (int l = 0; l < spec_.layers; ++l) {
@@ -117,6 +118,16 @@ DecoderRunner::DecoderRunner(std::shared_ptr<NativeContext> ctx, ModelSpec spec,
             kd_ = static_cast<uint16_t *>(alloc((size_t)max_context_ * kvd * 2));
             vd_ = static_cast<uint16_t *>(alloc((size_t)max_context_ * kvd * 2));
         }
+        if (eight_bit()) {
+            // a page is one block of 16 tokens
+            scales_ = static_cast<float *>(alloc(pool_pages * spec_.kv_heads * 2 * sizeof(float) * spec_.layers));
+            std::vector<int32_t> count((size_t)max_context_);
+            for (size_t i = 0; i < count.size(); ++i) count[i] = (int32_t)i;
+            count_ = static_cast<int32_t *>(alloc(count.size() * 4));
+            ctx_->check("upload positions", mslim_attn_buf_write(ctx_->handle(), count_, 0,
+                                                                 reinterpret_cast<const uint8_t *>(count.data()),
+                                                                 count.size() * 4));
+        }
         logits_ = static_cast<uint16_t *>(alloc((size_t)max_batch_ * spec_.vocab * 2));
         cold_.resize(max_batch_);
         cold_report_.assign(max_batch_, ColdReport{});
@@ -142,6 +153,22 @@ void *DecoderRunner::alloc(size_t bytes) {
     if (!p) throw NativeError("allocate runner buffer", 0, mslim_attn_last_error());
     owned_.push_back(p);
     return p;
+}
+
+mslim_attn_kv8_cache DecoderRunner::kv8_cache(int l, const int32_t *table) const {
+    static_assert(kPageTokens == 16, "a page is one block");
+    mslim_attn_kv8_cache c{};
+    c.pool_pages = (int64_t)max_batch_ * pages_per_seq_;
+    c.k_pool = k_pools_[l];
+    c.v_pool = v_pools_[l];
+    c.scales = scales_ + c.pool_pages * spec_.kv_heads * 2 * l;
+    c.page_table = table;
+    c.pages_per_seq = pages_per_seq_;
+    c.page_tokens = kPageTokens;
+    c.kv_heads = spec_.kv_heads;
+    c.head_dim = spec_.head_dim;
+    c.format = layout_ == KvLayout::PagedE4m3 ? MSLIM_ATTN_FORMAT_E4M3 : MSLIM_ATTN_FORMAT_INT8;
+    return c;
 }
 
 // Final norm, LM head and greedy token of `rows` hidden rows.
@@ -171,6 +198,18 @@ void DecoderRunner::chunk(int seq, const int32_t *ids, int n, int64_t prior) {
         ctx_->check("input norm + QKV projection",
                     mslim_attn_rmsnorm_gemm_qkv(h, w.input_norm, s.rms_eps, w.q, w.k, w.v, x_, q_, k_, v_, s.hidden,
                                                 qd, kvd, n));
+        if (eight_bit()) {
+            const mslim_attn_kv8_cache cache = kv8_cache(l, table_row(seq));
+            const int32_t before = (int32_t)prior;
+            ctx_->check("RoPE + K/V append",
+                        mslim_attn_rope_append_kv8(h, &cache, q_, k_, v_, qr_, 1, n, count_ + prior, s.q_heads,
+                                                   s.rope_theta, s.llama3, s.rope_factor, s.rope_low, s.rope_high,
+                                                   s.rope_original_max));
+            ctx_->check("causal attention",
+                        mslim_attn_prefill_kv8(h, &cache, qr_, attn_, 1, n, &before, s.q_heads, scale_));
+            mlp(w, n);
+            continue;
+        }
         ctx_->check("RoPE", mslim_attn_rope_qk(h, q_, qr_, k_, kr_, n, s.q_heads, s.kv_heads, s.head_dim, (int)prior,
                                                s.rope_theta, s.llama3, s.rope_factor, s.rope_low, s.rope_high,
                                                s.rope_original_max));
@@ -287,6 +326,20 @@ std::vector<Step> DecoderRunner::forward_batch(const std::vector<int32_t> &token
         for (int l = 0; l < s.layers; ++l) {
             const LayerWeights &w = w_.layers[l];
             injected_error(l);
+            if (eight_bit()) {
+                const mslim_attn_kv8_cache cache = kv8_cache(l, table_);
+                ctx_->check("input norm + QKV projection",
+                            mslim_attn_rmsnorm_gemm_qkv(h, w.input_norm, s.rms_eps, w.q, w.k, w.v, x_, q_, k_, v_,
+                                                        s.hidden, s.q_heads * s.head_dim, s.kv_heads * s.head_dim, b));
+                ctx_->check("RoPE + K/V append",
+                            mslim_attn_rope_append_kv8(h, &cache, q_, k_, v_, qr_, b, 1, pos_, s.q_heads, s.rope_theta,
+                                                       s.llama3, s.rope_factor, s.rope_low, s.rope_high,
+                                                       s.rope_original_max));
+                ctx_->check("8-bit attention",
+                            mslim_attn_decode_kv8(h, &cache, qr_, attn_, b, lens.data(), s.q_heads, scale_));
+                mlp(w, b);
+                continue;
+            }
             ctx_->check("input norm + QKV + RoPE + K/V append",
                         mslim_attn_rmsnorm_qkv_rope_append(h, w.input_norm, s.rms_eps, w.q, w.k, w.v, x_, qr_,
                                                            k_pools_[l], v_pools_[l], table_, pages_per_seq_,
@@ -562,6 +615,7 @@ void DecoderRunner::injected_error(int layer) {
 
 std::string DecoderRunner::logical_kv_sha256(int seq) const {
     ensure(seq >= 0 && seq < max_batch_, "sequence slot out of range");
+    ensure(!eight_bit(), "an 8-bit K/V layout has no exact K/V digest");
     check_healthy(seq);
     std::vector<const int32_t *> tables(spec_.layers, table_row(seq));
     std::vector<const void *> keys(k_pools_.begin(), k_pools_.end()), values(v_pools_.begin(), v_pools_.end());
@@ -613,7 +667,7 @@ void *mslim_model_new(void *attn_ctx, const mslim_model_spec *spec, const void *
     g_model_error.clear();
     try {
         mslim::ensure(attn_ctx && spec && weights, "null model arguments");
-        mslim::ensure(kv_layout == MSLIM_MODEL_KV_PAGED || kv_layout == MSLIM_MODEL_KV_DENSE, "unknown K/V layout");
+        mslim::ensure(kv_layout >= MSLIM_MODEL_KV_PAGED && kv_layout <= MSLIM_MODEL_KV_PAGED_INT8, "unknown K/V layout");
         mslim::model::ModelSpec s;
         s.layers = spec->layers;
         s.hidden = spec->hidden;

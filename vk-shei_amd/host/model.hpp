@@ -58,7 +58,8 @@ struct Step {
 // (the Workspace cache of load_dense_native_hip, mod.rs:308).  The two give
 // bit-identical tokens and logits, the reference's invariant of
 // mod.rs:2993-3048.
-enum class KvLayout { Paged = 0, Dense = 1 };
+// PagedE4m3, PagedInt8: 8-bit pages (mslim_attn_kv8_cache).
+enum class KvLayout { Paged = 0, Dense = 1, PagedE4m3 = 2, PagedInt8 = 3 };
 
 // ColdStore persistence of one slot: the reference's last_prefill_cold_seal_
 // seconds, last_deferred_cold_commit_seconds and last_deferred_cold_committed_
@@ -179,6 +180,9 @@ private:
     region::DevicePagePool all_layer_pool() const;
     std::vector<region::LayerBlocks> slot_blocks(int seq) const;
     void seal_slot(int seq, int64_t from, int64_t to);
+    bool eight_bit() const { return layout_ == KvLayout::PagedE4m3 || layout_ == KvLayout::PagedInt8; }
+    // Layer l's 8-bit cache under page-table rows `table`.
+    mslim_attn_kv8_cache kv8_cache(int l, const int32_t *table) const;
     void head(const uint16_t *rows_in, int rows);
     void mlp(const LayerWeights &w, int n);
     const int32_t *table_row(int seq) const { return table_ + (int64_t)seq * pages_per_seq_; }
@@ -206,6 +210,10 @@ private:
     const int32_t *cancel_ = nullptr;
     std::vector<char> poisoned_;
     int inject_kind_ = 0, inject_layer_ = -1;
+    // 8-bit layouts: block scales of every layer, and 0, 1, ... (the position
+    // of any chunk's first token, on the device)
+    float *scales_ = nullptr;
+    int32_t *count_ = nullptr;
     int32_t *table_ = nullptr, *pos_ = nullptr, *row_ids_ = nullptr;
     // one page-locked buffer: prompt or step ids, step positions, greedy tokens
     int32_t *io_ = nullptr, *ids_ = nullptr, *host_pos_ = nullptr, *next_ = nullptr;

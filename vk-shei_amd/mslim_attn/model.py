@@ -53,8 +53,8 @@ class ColdReport(C.Structure):
 
 LAYER_TENSORS = ("input_norm", "q", "k", "v", "o", "post_norm", "gate", "up", "down")
 
-# MSLIM_MODEL_KV_PAGED / MSLIM_MODEL_KV_DENSE
-KV_LAYOUTS = {"paged": 0, "dense": 1}
+# MSLIM_MODEL_KV_PAGED / _DENSE / _PAGED_E4M3 / _PAGED_INT8
+KV_LAYOUTS = {"paged": 0, "dense": 1, "paged_e4m3": 2, "paged_int8": 3}
 
 
 class Spec(C.Structure):
@@ -143,8 +143,9 @@ def _ids(values: Sequence[int]):
 
 class Model:
     """A decoder runner with `max_batch` sequence slots on a Context; K/V in
-    the ColdStore-exact paged pool ("paged") or dense token-major rows
-    ("dense").
+    the ColdStore-exact paged pool ("paged"), dense token-major rows ("dense")
+    or 8-bit pages ("paged_e4m3", "paged_int8": half the bytes per token, no
+    K/V digest and no ColdStore).
 
     `weights` maps "embed", "final_norm", "lm_head" and per layer l the names
     of LAYER_TENSORS ("layers.{l}.q", ...) to contiguous device BF16 tensors
