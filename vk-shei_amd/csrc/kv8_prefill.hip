@@ -60,6 +60,11 @@ __host__ __device__ inline int tiles_of(int prior, int queries, int tile_queries
     return (int)((end + kBN - 1) / kBN);
 }
 
+// Of a scale that the whole wavefront shares: a scalar test.
+__device__ __forceinline__ bool finite(float scale) {
+    return (__builtin_amdgcn_readfirstlane(__float_as_uint(scale)) & 0x7f800000u) != 0x7f800000u;
+}
+
 // First tile of workgroup w, and the workgroup that takes a tile.
 __device__ __forceinline__ int first_tile(const PrefillArgs &a, int w) { return w * a.share + min(w, a.extra); }
 __device__ __forceinline__ int owner_of(const PrefillArgs &a, int tile) {
@@ -77,7 +82,8 @@ __device__ __forceinline__ float2 *part_at(const PrefillArgs &a, int w, bool beg
 template <int FMT>
 __device__ __forceinline__ void widen_scaled(const u32x4_t &w, float scale, uint4 (&out)[2]) {
     uint32_t o[8];
-    if (FMT == kFormatE4m3 && (__float_as_uint(scale) & 0x7fffffu) == 0) {
+    if (FMT == kFormatE4m3 &&
+        __builtin_expect((__builtin_amdgcn_readfirstlane(__float_as_uint(scale)) & 0x7fffffu) == 0, 1)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, false));
@@ -211,26 +217,27 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
         };
         // The loaded tile to K stage ks and V stage vs.  V bytes behind the
         // last token, or of no page, become zeros; K's are masked.
+        // (Scales are the same for the wavefront, so their cases are branches.)
         auto store_k = [&](int ks) __attribute__((always_inline)) {
             if (!has_k) return;
-            // NaN where K's or V's scale is not finite
-            const float by = (scale.y - scale.y) + scale.x;
             uint4 w[2];
             widen_scaled<FMT>(k_in ? k_in_regs : u32x4_t{0, 0, 0, 0}, scale.x, w);
-            if (!(__builtin_fabsf(by) <= __FLT_MAX__)) w[0] = w[1] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+            if (!finite(scale.x) || !finite(scale.y))
+                w[0] = w[1] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
             *reinterpret_cast<uint4 *>(k_to0 + ks * kBN * DM) = w[0];
             *reinterpret_cast<uint4 *>(k_to1 + ks * kBN * DM) = w[1];
         };
         auto store_v = [&](int vs, int t) __attribute__((always_inline)) {
             if (!has_v) return;
-            uint4 w[2];
-            u32x4_t bytes = v_in && !no_page ? v_in_regs : u32x4_t{0, 0, 0, 0};
-            if (t * kBN + kBN > len) {
-                const int fill = min(max(len - (t * kBN + my_block * 16 + v_grp * 4), 0), 4);
-                bytes &= fill == 4 ? 0xffffffffu : (1u << (8 * fill)) - 1;
+            uint4 w[2] = {};
+            if (!no_page && finite(scale.y)) {
+                u32x4_t bytes = v_in ? v_in_regs : u32x4_t{0, 0, 0, 0};
+                if (__builtin_expect(t * kBN + kBN > len, 0)) {
+                    const int fill = min(max(len - (t * kBN + my_block * 16 + v_grp * 4), 0), 4);
+                    bytes &= fill == 4 ? 0xffffffffu : (1u << (8 * fill)) - 1;
+                }
+                widen_scaled<FMT>(bytes, scale.y, w);
             }
-            widen_scaled<FMT>(bytes, scale.y, w);
-            if (!(__builtin_fabsf(scale.y) <= __FLT_MAX__)) w[0] = w[1] = make_uint4(0, 0, 0, 0);
             *reinterpret_cast<uint4 *>(v_to + vs * kBN * DM) = w[0];
             *reinterpret_cast<uint4 *>(v_to + vs * kBN * DM + 8) = w[1];
         };
@@ -272,7 +279,7 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
         };
         // Key of element (kb, i) in its tile: kb * 32 + (i >> 2) * 8 + half * 4 + (i & 3).
         auto mask = [&](int t, const Pages &pg) __attribute__((always_inline)) {
-            if (t * kBN + kBN > common) {
+            if (__builtin_expect(t * kBN + kBN > common, 0)) {
                 const int most = limit - 1 - t * kBN - half * 4;
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
@@ -280,7 +287,7 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
                     for (int i = 0; i < 16; ++i)
                         if (kb * 32 + (i >> 2) * 8 + (i & 3) > most) s[kb][i] = -INFINITY;
             }
-            if (!all_known(pg)) {
+            if (__builtin_expect(!all_known(pg), 0)) {
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -311,7 +318,7 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
         // that is within the bound; else the rows whose maximum exceeds it
         // move it and the tile's P is taken again.
         auto settle = [&]() __attribute__((always_inline)) {
-            if (wave_any(!(psum <= kLazyBound))) {
+            if (__builtin_expect(wave_any(!(psum <= kLazyBound)), 0)) {
                 const float m_new = fmaxf(row_max(), m_used);
                 alpha = __builtin_amdgcn_exp2f(m_used - m_new);
                 l_run *= alpha;
@@ -451,50 +458,56 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
 
     // Workgroup -> run of tiles: XCD x (workgroups x, x + 8, ...) takes a
     // contiguous eighth of all, so the kv heads that it reads stay in its L2.
+    // One call of run() for all modes: a cold workgroup's time is the fetching
+    // of its instructions.
+    const int w = a.workgroups % kXcds || a.mode == kWhole
+                      ? (int)blockIdx.x
+                      : (int)(blockIdx.x % kXcds) * (a.workgroups / kXcds) + (int)(blockIdx.x / kXcds);
+    int b = 0, head, rt = 0, seg_begin = 0, tiles, at, end;
     if (a.mode == kWhole) {
-        const int rt = (int)(blockIdx.x % a.row_tiles), rest = (int)(blockIdx.x / a.row_tiles);
-        const int b = rest / c.kv_heads;
-        const int tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, rt);
-        run(b, rest % c.kv_heads, rt, 0, tiles, tiles, 0);
-        return;
-    }
-    const int w = a.workgroups % kXcds ? (int)blockIdx.x
-                                       : (int)(blockIdx.x % kXcds) * (a.workgroups / kXcds) + (int)(blockIdx.x / kXcds);
-    int at = a.mode == kPieces ? w : first_tile(a, w);
-    int b = 0;
-    for (int hi = a.batch - 1; b < hi;) {
-        const int mid = (b + hi + 1) >> 1;
-        if (a.begin[mid] <= at) b = mid;
-        else hi = mid - 1;
-    }
-    int head = (at - a.begin[b]) / a.per_head[b], rt = 0;
-    int seg_begin = a.begin[b] + head * a.per_head[b];
-    int tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, 0);
-    if (a.mode == kPieces) {
-        int pieces = (tiles + a.quota - 1) / a.quota;
+        rt = w % a.row_tiles;
+        head = w / a.row_tiles % c.kv_heads;
+        b = w / a.row_tiles / c.kv_heads;
+        tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, rt);
+        at = 0;
+        end = tiles;
+    } else {
+        at = a.mode == kPieces ? w : first_tile(a, w);
+        for (int hi = a.batch - 1; b < hi;) {
+            const int mid = (b + hi + 1) >> 1;
+            if (a.begin[mid] <= at) b = mid;
+            else hi = mid - 1;
+        }
+        head = (at - a.begin[b]) / a.per_head[b];
+        seg_begin = a.begin[b] + head * a.per_head[b];
+        tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, 0);
+        const int quota = a.mode == kPieces ? a.quota : 1;
+        int pieces = (tiles + quota - 1) / quota;
         while (seg_begin + pieces <= at) {
             seg_begin += pieces;
             tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, ++rt);
-            pieces = (tiles + a.quota - 1) / a.quota;
+            pieces = (tiles + quota - 1) / quota;
         }
-        const int i = at - seg_begin;
-        run(b, head, rt, i * tiles / pieces, (i + 1) * tiles / pieces, tiles, w);
-        if (tid == 0 && i == 0)
-            a.parts[(b * c.kv_heads + head) * a.row_tiles + rt] = Part{b, head, rt, w, pieces > 1 ? pieces : 0};
-        return;
-    }
-    const int end = first_tile(a, w + 1);
-    while (seg_begin + tiles <= at) {
-        seg_begin += tiles;
-        tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, ++rt);
+        if (a.mode == kPieces) {
+            const int i = at - seg_begin;
+            if (tid == 0 && i == 0)
+                a.parts[(b * c.kv_heads + head) * a.row_tiles + rt] = Part{b, head, rt, w, pieces > 1 ? pieces : 0};
+            seg_begin = 0;
+            at = i * tiles / pieces;
+            end = (i + 1) * tiles / pieces;
+        } else {
+            end = first_tile(a, w + 1);
+        }
     }
     Part begun = {};
-    for (bool again = false; at < end; again = true) {
-        if (again) __syncthreads();  // the LDS of the part before is free
+    for (;;) {
         const int tile = at - seg_begin, tile_end = min(tiles, end - seg_begin);
-        if (tile == 0 && tile_end < tiles) begun = Part{b, head, rt, w, owner_of(a, seg_begin + tiles - 1) - w + 1};
+        if (a.mode == kRuns && tile == 0 && tile_end < tiles)
+            begun = Part{b, head, rt, w, owner_of(a, seg_begin + tiles - 1) - w + 1};
         run(b, head, rt, tile, tile_end, tiles, w);
         at = seg_begin + tile_end;
+        if (at >= end) break;
+        __syncthreads();  // the LDS of this part is free
         seg_begin += tiles;
         if (++rt == a.row_tiles) {
             rt = 0;
@@ -505,7 +518,7 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
         }
         tiles = tiles_of(a.prior[b], a.queries, a.tile_queries, rt);
     }
-    if (tid == 0) a.parts[w] = begun;
+    if (a.mode == kRuns && tid == 0) a.parts[w] = begun;
 }
 
 // Merges the parts of a segment in the order of its keys: a wavefront per 32
