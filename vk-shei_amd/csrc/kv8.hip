@@ -832,8 +832,13 @@ __global__ __launch_bounds__(64 * WAVES, WGS) void attention_kernel(AttentionArg
         run(b, (int)(blockIdx.x % segments), 0, chunks_of(a.len[b], WAVES));
         return;
     }
-    int at = first_chunk(a, (int)blockIdx.x);
-    const int end = first_chunk(a, (int)blockIdx.x + 1);
+    // Row tiles of one kv head read the same bytes: they go to one XCD (that of
+    // workgroups x, x + 8, ...), which takes a contiguous eighth of all.
+    const int grid = (int)gridDim.x;
+    const int w = a.row_tiles > 1 && grid % 8 == 0 ? (int)(blockIdx.x % 8) * (grid / 8) + (int)(blockIdx.x / 8)
+                                                   : (int)blockIdx.x;
+    int at = first_chunk(a, w);
+    const int end = first_chunk(a, w + 1);
     for (bool again = false; at < end; again = true) {
         if (again) __syncthreads();  // the LDS of the part before is free
         int b = 0;
@@ -850,12 +855,21 @@ __global__ __launch_bounds__(64 * WAVES, WGS) void attention_kernel(AttentionArg
     }
 }
 
-// Tiles of 16 rows that a launch's workgroups take together: K and V are read
-// and widened once for all of them.
+// Bytes of K and V that a launch attends to.
+int64_t cache_bytes(const Kv8AttentionLaunch &l) {
+    int64_t tokens = 0;
+    for (int b = 0; b < l.batch; ++b) tokens += l.len[b];
+    return tokens * l.cache.kv_heads * l.cache.head_dim * 2;
+}
+
+// Tiles of 16 rows that a workgroup takes together.  Two read K and V once for
+// both, but leave a SIMD one wavefront's registers; one tile with the others in
+// workgroups of the same XCD reads them again from its caches, faster unless
+// they do not fit: 64 rows of 4 kv heads' groups after 4,000 tokens 32.8 (two)
+// and 21.4 us (one), 24 rows over 284 MB 88 and 109 us.
 int row_tiles_at_once(const Kv8AttentionLaunch &l) {
     const int64_t rows = (int64_t)l.queries * (l.q_heads / l.cache.kv_heads);
-    if (rows <= 16) return 1;
-    return rows <= 32 || l.cache.head_dim > 128 ? 2 : 4;
+    return rows > 16 && cache_bytes(l) >= kStreamBytes ? 2 : 1;
 }
 
 // How a launch runs.
@@ -877,8 +891,7 @@ void launch_attention(const AttentionArgs &a, const Shape &s, unsigned grid, hip
         else if (s.nt == 1 && s.waves == 8) MSLIM_KV8_LAUNCH(1, 8, 1, false);
         else if (s.nt == 1 && s.stream) MSLIM_KV8_LAUNCH(1, 4, 2, true);
         else if (s.nt == 1) MSLIM_KV8_LAUNCH(1, 4, 2, false);
-        else if (s.nt == 2) MSLIM_KV8_LAUNCH(2, 4, 1, false);
-        else MSLIM_KV8_LAUNCH(4, 4, 1, false);
+        else MSLIM_KV8_LAUNCH(2, 4, 1, false);
     } else {
         if (s.nt == 1) MSLIM_KV8_LAUNCH(1, 4, 1, false);
         else MSLIM_KV8_LAUNCH(2, 4, 1, false);
@@ -973,7 +986,7 @@ Shape shape_of(const Kv8AttentionLaunch &l) {
     }
     const int64_t parts = s.workgroups / (s.segments * l.batch) + 1;
     s.merge_launch = parts * std::min<int64_t>(rows, 16 * s.nt) * (l.cache.head_dim + 2) * 4 > kMergeLaunchBytes;
-    s.stream = s.total * s.waves * kTile * l.cache.head_dim * 2 >= kStreamBytes;
+    s.stream = s.row_tiles == 1 && cache_bytes(l) >= kStreamBytes;
     return s;
 }
 }  // namespace
