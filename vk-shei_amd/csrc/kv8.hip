@@ -615,7 +615,9 @@ __global__ __launch_bounds__(64 * WAVES, WGS) void attention_kernel(AttentionArg
         // Loads never branch: a block past the end repeats the last one, an
         // entry that names no page reads page 0, a piece past head_dim the
         // row's last one; what they bring is masked below.
-        const int t_first = ch * CHUNK + wave * kTile, t_end = min(len, ch_end * CHUNK);
+        // no row of the tile sees more than its last one
+        const int most = len - a.queries + min(rt * ROWS + ROWS - 1, rows - 1) / group + 1;
+        const int t_first = ch * CHUNK + wave * kTile, t_end = min(min(len, most), ch_end * CHUNK);
         const int32_t *table = c.table + (int64_t)b * c.pages_per_seq;
         const int last = max(len - 1, 0) & ~15;
         const int in_page = (1 << c.shift) - 1;
@@ -994,8 +996,13 @@ Shape shape_of(const Kv8AttentionLaunch &l) {
 Kv8AttentionPlan kv8_attention_plan(const Kv8AttentionLaunch &l) {
     const Shape s = shape_of(l);
     Kv8AttentionPlan p{};
-    // as even without where segments are many; positions of chunks are 32 bits
-    if (s.segments * l.batch > 4 * s.workgroups || s.total > INT32_MAX / 2) return p;
+    // Segments enough for every workgroup and none much longer than a
+    // workgroup's share are as even unsplit, with nothing to merge: 333 queries
+    // after 777 tokens, groups of seven, 35.6 -> 27.7 us.
+    int longest = 0;
+    for (int b = 0; b < l.batch; ++b) longest = std::max(longest, chunks_of(l.len[b], s.waves));
+    if (s.segments * l.batch >= s.workgroups && 2 * s.workgroups * longest <= 3 * s.total) return p;
+    if (s.total > INT32_MAX / 2) return p;  // positions of chunks are 32 bits
     p.split = true;
     p.partial_bytes = (size_t)(2 * s.workgroups) * 16 * s.nt * (l.cache.head_dim + 2) * sizeof(float);
     p.counters = (size_t)(s.segments * l.batch);

@@ -641,19 +641,19 @@ void launch(const PrefillArgs &a, unsigned grid, hipStream_t stream) {
 }  // namespace
 
 // The other kernel takes 16 rows and 32 tokens a step, on 2,048 wavefronts at
-// once; up to about eleven steps of each it is done before this one's fixed
-// 10 us and its merge are made up for: 256 queries after 1,000 tokens, 32/8
-// heads, ten steps, 19 and 30 us; 200 after 3,000, twenty steps, 46 and 36 us.
-// Up to 64 rows a kv head most of a workgroup here would idle: 8 queries of 32
-// sessions, 64/8 heads, 167 and 249 us.
+// once, 2 us each; up to about fourteen steps it is done before this one's
+// fixed 10 us and its merge are made up for: 256 queries after 1,000 tokens,
+// 32/8 heads, nine steps, 18 and 30 us; 200 after 3,000, nineteen steps, 46
+// and 36 us.  Up to 64 rows a kv head most of a workgroup here would idle: 8
+// queries of 32 sessions, 64/8 heads, 161 and 249 us.
 bool kv8_prefill_supported(const Kv8AttentionLaunch &l) {
     const int group = l.q_heads / l.cache.kv_heads;
     const int64_t rows = (int64_t)l.queries * group;
     if (l.cache.head_dim > 128 || group > kRows || rows <= 64) return false;
     double steps = 0.0;
     for (int b = 0; b < l.batch; ++b)
-        steps += (double)((rows + 15) / 16) * ((l.len[b] + 31) / 32) * l.cache.kv_heads;
-    return steps > 11 * 2048;
+        steps += (double)((rows + 15) / 16) * ((l.len[b] - l.queries / 2 + 31) / 32) * l.cache.kv_heads;
+    return steps > 14 * 2048;
 }
 
 namespace {
