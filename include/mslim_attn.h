@@ -111,8 +111,8 @@ int mslim_attn_ctx_set_stream(void *ctx, void *hip_stream);
  * threads on two streams at once.
  *
  * Calls recorded into a graph.  A recorded call keeps the addresses of the
- * context buffers that it uses: decode and its portable form their split
- * partials and counters, a prefill its split partials or pool counter,
+ * context buffers that it uses: decode, its portable form and the 8-bit
+ * attention their split partials and counters, a prefill its split partials or pool counter,
  * products of more than 16 token rows their split partials, the fused RMSNorm
  * entry points their normalised and Q/K/V rows, RoPE its cos/sin table.
  *   * The addresses stay valid until mslim_attn_ctx_destroy: a call that needs
@@ -125,8 +125,8 @@ int mslim_attn_ctx_set_stream(void *ctx, void *hip_stream);
  *     is not replayed after the context ran another.
  *   * Nothing can be allocated while recording.  A call whose buffers are not
  *     there yet fails, except where it can run without: a prefill of a group
- *     other than 1, 2 or a multiple of 4 and a portable decode run unsplit,
- *     and so do products, to the same bits. */
+ *     other than 1, 2 or a multiple of 4, a portable decode and the 8-bit
+ *     attention run unsplit, and so do products, to the same bits. */
 
 /* Context options.  No reference counterpart (the OpenCL engine has no merge
  * choice); for tests and callers that want the two-launch merge.
@@ -454,7 +454,12 @@ int mslim_attn_logical_kv_sha256(void *ctx, int layers, int64_t tokens, int kv_h
  * 16-byte.  The table is device memory, as are the positions; an entry that
  * names no page of the pool (padding, -1) is allowed: nothing is written
  * through it, rows read through it are zeros, and attention gives its tokens
- * no weight. */
+ * no weight.  A table row names fewer than 2^31 - 4096 tokens.
+ * A pool needs no clearing where sequences begin at a block's first token.
+ * Where bytes and scales are put there by something else than an append, the
+ * scales are powers of two (the attention is exact for these) and no token of
+ * a sequence has an E4M3 NaN byte (0x7f, 0xff) in V: rows of a prefill before
+ * that token could see it. */
 #define MSLIM_ATTN_FORMAT_E4M3 4
 #define MSLIM_ATTN_FORMAT_INT8 5
 typedef struct {
@@ -486,8 +491,8 @@ typedef struct {
  *   A value that is not finite makes its block's scale NaN: attention that
  *   sees the block gives NaN until an append begins the block anew.
  * A row at a position outside [0, pages_per_seq * page_tokens) is not stored.
- * Sequences of one call must not share the pages they append to.  q_out must
- * not alias an input.  batch at most MSLIM_ATTN_MAX_BATCH, batch * tokens at
+ * No page that is appended to may stand twice in the rows of the table, be it
+ * in one sequence's or in two.  q_out must not alias an input.  batch at most MSLIM_ATTN_MAX_BATCH, batch * tokens at
  * most 2^22. */
 int mslim_attn_rope_append_kv8(void *ctx, const mslim_attn_kv8_cache *cache, const void *q, const void *k,
                                const void *v, void *q_out, int batch, int tokens, const int32_t *positions,

@@ -34,7 +34,8 @@ BAD_CACHE = [dict(k_pool=0), dict(v_pool=0), dict(scales=0), dict(page_table=0),
              dict(pool_pages=1 << 31), dict(pages_per_seq=0), dict(page_tokens=8), dict(page_tokens=24),
              dict(page_tokens=8192), dict(kv_heads=0), dict(kv_heads=16385), dict(head_dim=8), dict(head_dim=72),
              dict(head_dim=272), dict(format=3), dict(format=6), dict(k_pool=A + 8), dict(v_pool=A + 4),
-             dict(scales=A + 4), dict(pages_per_seq=1 << 27)]
+             dict(scales=A + 4), dict(pages_per_seq=1 << 27),
+             dict(pages_per_seq=(1 << 27) - 256)]
 
 
 @pytest.mark.parametrize("bad", BAD_CACHE, ids=str)

@@ -1180,8 +1180,9 @@ static int kv8_cache(const mslim_attn_kv8_cache *cache, int batch, mslim::Kv8Cac
         cache->pool_pages > INT32_MAX)
         return fail("8-bit cache needs 1..16384 kv_heads, pages_per_seq >= 1 and 1..2^31-1 pool_pages");
     if (cache->reserved != 0) return fail("8-bit cache: reserved must be 0");
-    if ((int64_t)cache->pages_per_seq * cache->page_tokens > INT32_MAX - 64)
-        return fail("8-bit cache: the page table names more than 2^31 tokens");
+    // Tokens are counted in 32 bits, by steps that go up to two chunks past the end.
+    if ((int64_t)cache->pages_per_seq * cache->page_tokens > INT32_MAX - 4096)
+        return fail("8-bit cache: a page table row names more than 2^31 - 4097 tokens");
     if (!aligned(cache->k_pool, 16) || !aligned(cache->v_pool, 16) || !aligned(cache->scales, 8))
         return fail("8-bit cache needs 16-byte aligned pools and 8-byte aligned scales");
     if (batch < 1 || batch > MSLIM_ATTN_MAX_BATCH) return fail("8-bit cache batch must be 1..4096");

