@@ -89,7 +89,9 @@ def inputs(seed, batch, queries, qh, d):
 CHUNKS = [
     (32, 8, 128, 16, [3584], 512), (28, 4, 128, 64, [777, 2000, 0], 700), (6, 6, 96, 16, [1500, 0, 64, 2999], 1001),
     (16, 2, 64, 32, [100] * 20, 300), (64, 8, 128, 16, [2000, 1], 1025), (60, 3, 48, 4096, [999] * 3, 600),
-    (256, 1, 16, 16, [700], 200), (200, 1, 112, 128, [500, 3], 150), (16, 2, 64, 16, [90, 300] * 35, 100)]
+    (256, 1, 16, 16, [700], 200), (200, 1, 112, 128, [500, 3], 150), (16, 2, 64, 16, [90, 300] * 35, 100),
+    # two tiles of 16 rows at once: segments alike, ragged ones, head_dim over 128
+    (32, 8, 128, 16, [300], 512), (12, 6, 96, 16, [5, 500, 40] * 16, 50), (16, 8, 256, 16, [77] * 6, 90)]
 
 
 @pytest.mark.parametrize("fmt", [E4M3, INT8])

@@ -378,6 +378,7 @@ constexpr int kMergeParts = 16;          // parts that a merging thread loads at
 // non-temporally: 538 MB 99.8 -> 92.0 us, 269 MB 53.2 -> 51.0 us, 67 MB
 // 20.0 -> 22.1 us.
 constexpr int64_t kStreamBytes = 200ll << 20;
+constexpr int64_t kRereadBytes = 100ll << 20;  // kv8_two_row_tiles
 // A segment's parts above these bytes merge in a launch of their own, a
 // workgroup per row, instead of in the workgroup that ends last, to which the
 // device's memory gives about 25 GB/s: eight rows of four heads after 8,000
@@ -864,16 +865,6 @@ int64_t cache_bytes(const Kv8AttentionLaunch &l) {
     return tokens * l.cache.kv_heads * l.cache.head_dim * 2;
 }
 
-// Tiles of 16 rows that a workgroup takes together.  Two read K and V once for
-// both, but leave a SIMD one wavefront's registers; one tile with the others in
-// workgroups of the same XCD reads them again from its caches, faster unless
-// they do not fit: 64 rows of 4 kv heads' groups after 4,000 tokens 32.8 (two)
-// and 21.4 us (one), 24 rows over 284 MB 88 and 109 us.
-int row_tiles_at_once(const Kv8AttentionLaunch &l) {
-    const int64_t rows = (int64_t)l.queries * (l.q_heads / l.cache.kv_heads);
-    return rows > 16 && cache_bytes(l) >= kStreamBytes ? 2 : 1;
-}
-
 // How a launch runs.
 struct Shape {
     int nt, waves;  // row tiles of 16 at once, wavefronts of a workgroup
@@ -893,7 +884,8 @@ void launch_attention(const AttentionArgs &a, const Shape &s, unsigned grid, hip
         else if (s.nt == 1 && s.waves == 8) MSLIM_KV8_LAUNCH(1, 8, 1, false);
         else if (s.nt == 1 && s.stream) MSLIM_KV8_LAUNCH(1, 4, 2, true);
         else if (s.nt == 1) MSLIM_KV8_LAUNCH(1, 4, 2, false);
-        else MSLIM_KV8_LAUNCH(2, 4, 1, false);
+        else if (s.stream) MSLIM_KV8_LAUNCH(2, 4, 2, true);
+        else MSLIM_KV8_LAUNCH(2, 4, 2, false);
     } else {
         if (s.nt == 1) MSLIM_KV8_LAUNCH(1, 4, 1, false);
         else MSLIM_KV8_LAUNCH(2, 4, 1, false);
@@ -923,6 +915,21 @@ void launch_append(const AppendArgs &a, bool rotate, unsigned grid, hipStream_t 
 }
 
 }  // namespace
+
+// Two tiles read and widen K and V once for both: 0.9 instead of 1.2 us per 16
+// rows and 32 tokens on every wavefront.  But there are half as many segments,
+// so parts are twice as large where these are cut: it pays where the segments
+// fill the device without that (512 queries after 512 tokens, 32/8 heads, 27.4
+// -> 22.5 us; 256 after 1,000, half as many, 17.7 -> 23.9), or where the
+// second reading by workgroups of the same XCD no longer comes from the caches
+// (20 rows of 16 sessions, 98 MB 29.0 and 29.6 us, of 32 of 284 MB 86 -> 74; 64
+// rows of 16, 131 MB, 78 -> 50).
+bool kv8_two_row_tiles(const Kv8AttentionLaunch &l) {
+    const int64_t rows = (int64_t)l.queries * (l.q_heads / l.cache.kv_heads);
+    if (rows <= 16) return false;
+    const int64_t segments = (rows + 31) / 32 * l.cache.kv_heads * l.batch;
+    return segments >= (l.cache.head_dim > 128 ? kCus : 2 * kCus) || cache_bytes(l) >= kRereadBytes;
+}
 
 namespace {
 // 16-token blocks that a sequence's rows can reach, and workgroups of a block
@@ -968,7 +975,7 @@ hipError_t launch_kv8_gather(const Kv8Cache &cache, int batch, int tokens, const
 namespace {
 Shape shape_of(const Kv8AttentionLaunch &l) {
     Shape s;
-    s.nt = row_tiles_at_once(l);
+    s.nt = kv8_two_row_tiles(l) ? 2 : 1;
     const int64_t rows = (int64_t)l.queries * (l.q_heads / l.cache.kv_heads);
     s.row_tiles = (int)((rows + 16 * s.nt - 1) / (16 * s.nt));
     s.segments = (int64_t)l.cache.kv_heads * s.row_tiles;
@@ -980,7 +987,7 @@ Shape shape_of(const Kv8AttentionLaunch &l) {
     s.waves = 4;
     s.total = chunks(4);
     const bool wide = l.cache.head_dim > 128;
-    s.workgroups = std::min<int64_t>(s.total, s.nt == 1 && !wide ? 2 * kCus : kCus);
+    s.workgroups = std::min<int64_t>(s.total, wide ? kCus : 2 * kCus);
     if (s.nt == 1 && !wide && s.workgroups >= kWideParts * s.segments * l.batch) {
         s.waves = 8;
         s.total = chunks(8);
