@@ -114,7 +114,8 @@ LONG = [
     (32, 8, 128, 16, [25600] * 5, 1), (32, 8, 128, 64, list(range(300, 7100, 200)), 1), (28, 4, 112, 16, [31000] * 8, 1),
     (28, 4, 112, 16, list(range(1000, 15000, 500)) + [40000], 1), (32, 8, 128, 16, [25600] * 5, 5),
     (32, 8, 128, 16, [25601, 30000, 17, 70000], 12), (32, 8, 128, 32, [3000] * 40, 5), (8, 2, 256, 16, [53000] * 4, 6),
-    (5, 1, 208, 16, [131000] * 4, 9), (20, 5, 80, 16, [70000, 69999, 71003, 70000], 7), (16, 8, 64, 16, [60000] * 4, 9)]
+    (5, 1, 208, 16, [131000] * 4, 9), (20, 5, 80, 16, [70000, 69999, 71003, 70000], 7), (16, 8, 64, 16, [60000] * 4, 9),
+    (32, 8, 128, 16, list(range(500, 8000, 230)), 5), (24, 8, 112, 64, list(range(500, 8000, 230)), 6)]
 
 
 @pytest.mark.parametrize("fmt", [E4M3, INT8])

@@ -396,6 +396,8 @@ struct Kv8AttentionPlan {
 };
 Kv8AttentionPlan kv8_attention_plan(const Kv8AttentionLaunch &l);
 hipError_t launch_kv8_attention(const Kv8AttentionLaunch &l, hipStream_t stream);
+// Its steps of 16 rows and 32 tokens.
+double kv8_steps(const Kv8AttentionLaunch &l);
 // Whether a workgroup of that launch takes two tiles of 16 rows at once.
 bool kv8_two_row_tiles(const Kv8AttentionLaunch &l);
 // The same for many rows (csrc/kv8_prefill.hip): bound by its matrix products

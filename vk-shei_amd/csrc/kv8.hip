@@ -378,15 +378,11 @@ constexpr int kMergeParts = 16;          // parts that a merging thread loads at
 // non-temporally: 538 MB 99.8 -> 92.0 us, 269 MB 53.2 -> 51.0 us, 67 MB
 // 20.0 -> 22.1 us.
 constexpr int64_t kStreamBytes = 200ll << 20;
-constexpr int64_t kRereadBytes = 100ll << 20;  // kv8_two_row_tiles
-// A segment's parts above these bytes merge in a launch of their own, a
-// workgroup per row, instead of in the workgroup that ends last, to which the
-// device's memory gives about 25 GB/s: eight rows of four heads after 8,000
-// tokens, 530 KB a segment, 35.3 -> 19.7 us; at 66 KB (one row of four heads)
-// 13.5 and 12.3 us, at 33 KB equal.
-constexpr int64_t kMergeLaunchBytes = 64 << 10;
-// Workgroups of eight wavefronts, one per CU, instead of four, two per CU,
-// where segments have at least this many parts: half as many to merge (8,192
+// kv8_two_row_tiles
+constexpr int64_t kRereadBytes = 100ll << 20;
+constexpr int64_t kPairSteps = 9 * 2048;
+// One row tile: workgroups of eight wavefronts, one per CU, instead of four, two
+// per CU, where segments have at least this many parts: half as many to merge (8,192
 // tokens, 64 parts: 19.8 -> 13.5 us; 4 x 32,768 56.5 -> 53.2 us).  With
 // several segments to a workgroup the switch from one to the next stalls
 // twice the wavefronts: 32 sequences of 512 .. 8,192 tokens 63 -> 68 us.
@@ -884,6 +880,8 @@ void launch_attention(const AttentionArgs &a, const Shape &s, unsigned grid, hip
         else if (s.nt == 1 && s.waves == 8) MSLIM_KV8_LAUNCH(1, 8, 1, false);
         else if (s.nt == 1 && s.stream) MSLIM_KV8_LAUNCH(1, 4, 2, true);
         else if (s.nt == 1) MSLIM_KV8_LAUNCH(1, 4, 2, false);
+        else if (s.waves == 8 && s.stream) MSLIM_KV8_LAUNCH(2, 8, 1, true);
+        else if (s.waves == 8) MSLIM_KV8_LAUNCH(2, 8, 1, false);
         else if (s.stream) MSLIM_KV8_LAUNCH(2, 4, 2, true);
         else MSLIM_KV8_LAUNCH(2, 4, 2, false);
     } else {
@@ -916,19 +914,50 @@ void launch_append(const AppendArgs &a, bool rotate, unsigned grid, hipStream_t 
 
 }  // namespace
 
+// Whether segments (`per` of each sequence) of workgroups of `waves`
+// wavefronts are as even uncut: enough for `slots` workgroups at once and none
+// much longer than its share.  There is nothing to merge then: 333 queries
+// after 777 tokens, groups of seven, 35.6 -> 27.7 us.
+static bool even_uncut(const Kv8AttentionLaunch &l, int64_t per, int waves, int64_t slots) {
+    int64_t total = 0, longest = 0;
+    for (int b = 0; b < l.batch; ++b) {
+        const int64_t n = chunks_of(l.len[b], waves);
+        total += n * per;
+        longest = std::max(longest, n);
+    }
+    slots = std::min(slots, total);
+    return per * l.batch >= slots && 2 * slots * longest <= 3 * total;
+}
+
 // Two tiles read and widen K and V once for both: 0.9 instead of 1.2 us per 16
 // rows and 32 tokens on every wavefront.  But there are half as many segments,
-// so parts are twice as large where these are cut: it pays where the segments
-// fill the device without that (512 queries after 512 tokens, 32/8 heads, 27.4
-// -> 22.5 us; 256 after 1,000, half as many, 17.7 -> 23.9), or where the
-// second reading by workgroups of the same XCD no longer comes from the caches
-// (20 rows of 16 sessions, 98 MB 29.0 and 29.6 us, of 32 of 284 MB 86 -> 74; 64
-// rows of 16, 131 MB, 78 -> 50).
+// and what is cut has parts twice as large.  It pays
+//   * where segments fill the device, two workgroups of four wavefronts per
+//     CU: 512 queries after 512 tokens, 32/8 heads, 27.2 -> 22.6 us;
+//   * where caches do not serve the second reading: five queries of 48
+//     sessions, 188 MB, 59 -> 52 us, of 32 ragged ones, 284 MB, 86 -> 74;
+//   * where there are nine steps or more (of 16 rows) to make up for the merge
+//     and workgroups of eight wavefronts take one segment each, or cut few into
+//     many parts: 16 queries of 8 sessions after 8,000 tokens 61 -> 45 us, 256
+//     of one after 2,500 31.6 -> 27.5; but of 4 sessions after 4,000, eight
+//     steps, 21.9 and 22.3, 5 after 20,000, five steps, 20 and 24, and 333 after
+//     777, 28/4 heads, 292 segments on 256 CUs, 23 and 27.
+// Over 128 dims a CU holds one workgroup of four wavefronts either way.
 bool kv8_two_row_tiles(const Kv8AttentionLaunch &l) {
     const int64_t rows = (int64_t)l.queries * (l.q_heads / l.cache.kv_heads);
     if (rows <= 16) return false;
-    const int64_t segments = (rows + 31) / 32 * l.cache.kv_heads * l.batch;
-    return segments >= (l.cache.head_dim > 128 ? kCus : 2 * kCus) || cache_bytes(l) >= kRereadBytes;
+    const bool wide = l.cache.head_dim > 128;
+    const int64_t per = (rows + 31) / 32 * l.cache.kv_heads, segments = per * l.batch;
+    if (segments >= (wide ? kCus : 2 * kCus) || cache_bytes(l) >= kRereadBytes) return true;
+    return !wide && kv8_steps(l) > kPairSteps &&
+           (segments <= kCus / 2 || (segments <= kCus && even_uncut(l, per, 8, kCus)));
+}
+
+double kv8_steps(const Kv8AttentionLaunch &l) {
+    const int64_t tiles = ((int64_t)l.queries * (l.q_heads / l.cache.kv_heads) + 15) / 16;
+    double steps = 0.0;
+    for (int b = 0; b < l.batch; ++b) steps += (double)((l.len[b] - l.queries / 2 + kTile - 1) / kTile);
+    return steps * (double)tiles * l.cache.kv_heads;
 }
 
 namespace {
@@ -984,17 +1013,30 @@ Shape shape_of(const Kv8AttentionLaunch &l) {
         for (int b = 0; b < l.batch; ++b) n += chunks_of(l.len[b], waves) * s.segments;
         return n;
     };
+    const int64_t all = s.segments * l.batch;
+    const bool wide = l.cache.head_dim > 128;
     s.waves = 4;
     s.total = chunks(4);
-    const bool wide = l.cache.head_dim > 128;
     s.workgroups = std::min<int64_t>(s.total, wide ? kCus : 2 * kCus);
-    if (s.nt == 1 && !wide && s.workgroups >= kWideParts * s.segments * l.batch) {
+    // Two row tiles: workgroups of eight wavefronts where none goes on from one
+    // segment to the next, or few do: five rows of 32 sessions of 8,000 tokens
+    // 109 -> 90 us, of 32 ragged ones 74 -> 86.
+    const bool eight = s.nt == 2 ? all <= kCus / 2 || (all < 2 * kCus && even_uncut(l, s.segments, 8, kCus))
+                                 : s.workgroups >= kWideParts * all;
+    if (!wide && eight) {
         s.waves = 8;
         s.total = chunks(8);
         s.workgroups = std::min<int64_t>(s.total, kCus);
     }
-    const int64_t parts = s.workgroups / (s.segments * l.batch) + 1;
-    s.merge_launch = parts * std::min<int64_t>(rows, 16 * s.nt) * (l.cache.head_dim + 2) * 4 > kMergeLaunchBytes;
+    // The workgroup that ends last merges a segment's parts at about 25 GB/s,
+    // one of many at that; a launch of a workgroup per row takes 2 us and
+    // another for every 512 of them: eight rows of four heads after 8,000
+    // tokens, 530 KB a segment, 35.3 (fused) and 19.7 us, 66 KB of one row of
+    // four heads 13.5 and 12.3, 83 KB of 32 rows of each of 64 segments 22.3
+    // and 27.7.
+    const int64_t parts = s.workgroups / all + 1;
+    const double part_kb = (double)(parts * std::min<int64_t>(rows, 16 * s.nt) * (l.cache.head_dim + 2)) * 4 / 1024;
+    s.merge_launch = part_kb * 0.04 > 2.0 + (double)(all * 16 * s.nt) / 512;
     s.stream = s.row_tiles == 1 && cache_bytes(l) >= kStreamBytes;
     return s;
 }
@@ -1003,12 +1045,7 @@ Shape shape_of(const Kv8AttentionLaunch &l) {
 Kv8AttentionPlan kv8_attention_plan(const Kv8AttentionLaunch &l) {
     const Shape s = shape_of(l);
     Kv8AttentionPlan p{};
-    // Segments enough for every workgroup and none much longer than a
-    // workgroup's share are as even unsplit, with nothing to merge: 333 queries
-    // after 777 tokens, groups of seven, 35.6 -> 27.7 us.
-    int longest = 0;
-    for (int b = 0; b < l.batch; ++b) longest = std::max(longest, chunks_of(l.len[b], s.waves));
-    if (s.segments * l.batch >= s.workgroups && 2 * s.workgroups * longest <= 3 * s.total) return p;
+    if (even_uncut(l, s.segments, s.waves, l.cache.head_dim > 128 || s.waves == 8 ? kCus : 2 * kCus)) return p;
     if (s.total > INT32_MAX / 2) return p;  // positions of chunks are 32 bits
     p.split = true;
     p.partial_bytes = (size_t)(2 * s.workgroups) * 16 * s.nt * (l.cache.head_dim + 2) * sizeof(float);

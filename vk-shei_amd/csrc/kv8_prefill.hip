@@ -642,20 +642,17 @@ void launch(const PrefillArgs &a, unsigned grid, hipStream_t stream) {
 
 // The other kernel takes 16 rows and 32 tokens a step, on 2,048 wavefronts at
 // once, 1.2 us each or, two row tiles at a time, 0.9 us; this one's 0.5 us per
-// such step have to make up for its fixed 26 us.  E4M3: 256 queries after 2,000
-// tokens, 32/8 heads, seventeen steps, 27 us there and 35 here; 333 after 1,777,
-// 28/4 heads, as many, 36 and 33; two at a time 512 after 1,024, twenty, 30 and
-// 36; 600 after 1,200, 28/4 heads, 24, 45 and 37.  Up to 64 rows a kv head most
-// of a workgroup here would idle: 8 queries of 32 sessions, 64/8 heads, 117 and
-// 249 us.
+// such step have to make up for its fixed 26 us.  E4M3: 400 queries after 1,000
+// tokens, 32/8 heads, 15 steps, 32 us there and 33 here; 333 after 1,777, 28/4
+// heads, 17 steps, 37 and 32; two at a time 512 after 1,024, 20 steps, 30 and
+// 35; 1,024 after 256, 24 steps, 43 and 40; 256 after 4,000, 32 steps, still 38
+// and 41.  Up to 64 rows a kv head most of a workgroup here would idle: 8
+// queries of 32 sessions, 64/8 heads, 117 and 249 us.
 bool kv8_prefill_supported(const Kv8AttentionLaunch &l) {
     const int group = l.q_heads / l.cache.kv_heads;
     const int64_t rows = (int64_t)l.queries * group;
     if (l.cache.head_dim > 128 || group > kRows || rows <= 64) return false;
-    double steps = 0.0;
-    for (int b = 0; b < l.batch; ++b)
-        steps += (double)((rows + 15) / 16) * ((l.len[b] - l.queries / 2 + 31) / 32) * l.cache.kv_heads;
-    return steps > (kv8_two_row_tiles(l) ? 24 : 18) * 2048;
+    return kv8_steps(l) > (kv8_two_row_tiles(l) ? 24 : 16) * 2048;
 }
 
 namespace {
