@@ -1026,7 +1026,13 @@ Shape shape_of(const Kv8AttentionLaunch &l) {
     if (!wide && eight) {
         s.waves = 8;
         s.total = chunks(8);
-        s.workgroups = std::min<int64_t>(s.total, kCus);
+        // no more workgroups, in eights for the XCDs, than take the longest
+        // share: fewer parts in the same time (one of 20,000 tokens 17.8 ->
+        // 16.7 us; of workgroups of four wavefronts, two per CU, the CU's
+        // other one hides the longer shares: 32 of 100 .. 1,000 tokens 17.4
+        // and 18.3)
+        const int64_t share = (s.total + kCus - 1) / kCus;
+        s.workgroups = std::min<int64_t>(((s.total + share - 1) / share + 7) / 8 * 8, std::min<int64_t>(s.total, kCus));
     }
     // The workgroup that ends last merges a segment's parts at about 25 GB/s,
     // one of many at that; a launch of a workgroup per row takes 2 us and
