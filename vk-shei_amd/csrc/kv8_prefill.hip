@@ -493,8 +493,8 @@ __global__ __launch_bounds__(512, 1) void kv8_prefill_kernel(PrefillArgs a) {
             if (tid == 0 && i == 0)
                 a.parts[(b * c.kv_heads + head) * a.row_tiles + rt] = Part{b, head, rt, w, pieces > 1 ? pieces : 0};
             seg_begin = 0;
-            at = (int)((int64_t)i * tiles / pieces);
-            end = (int)((int64_t)(i + 1) * tiles / pieces);
+            at = i * (tiles / pieces) + min(i, tiles % pieces);
+            end = (i + 1) * (tiles / pieces) + min(i + 1, tiles % pieces);
         } else {
             end = first_tile(a, w + 1);
         }
