@@ -41,7 +41,7 @@ struct PrefillArgs {
     int tile_queries;  // queries of a row tile: kRows / group
     int row_tiles;
     float scale_log2e;
-    // Segments (sequence, kv head, row tile) laid end to end, by MODE:
+    // Segments (sequence, kv head, row tile) laid end to end, by mode:
     //   kWhole   a workgroup per segment;
     //   kPieces  a workgroup per piece of a segment, of `quota` tiles at most;
     //   kRuns    workgroup w takes `share` tiles (one more for the first
